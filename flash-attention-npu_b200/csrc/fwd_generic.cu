@@ -13,6 +13,7 @@
 #include <cstring>
 #include "fa_utils.cuh"
 #include "fa_internal.h"
+#include "tree_mask.cuh"
 
 namespace fa {
 
@@ -24,9 +25,13 @@ struct FwdArgs {
     float* o_part;
     float* lse_part;
     int part_minus_inf;   // partial LSE of an empty range is -inf (else final +inf)
+    TreeMask tree;        // TREE instantiation
+    int min_split_keys;
 };
 
-template <typename T, int HD>
+// TREE: the queries are a tree of drafted tokens behind the cached rows (tree_mask.cuh).  q is the stacked copy that the
+// preparing kernel leaves, (batch, KV head, token x group, dim), and the keys of a split are worked out here from the length.
+template <typename T, int HD, bool TREE>
 __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
     constexpr int BM = kGenericBM, BN = kGenericBN;
     constexpr int PITCH = HD * 2;
@@ -45,7 +50,11 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
     int q_off = 0, sq = p.sq, k_off = 0, sk = p.sk;
     if (p.cu_seqlens_q) { q_off = p.cu_seqlens_q[b]; sq = p.cu_seqlens_q[b + 1] - q_off; }
     if (p.cu_seqlens_k) { k_off = p.cu_seqlens_k[b]; sk = p.cu_seqlens_k[b + 1] - k_off; }
-    if (p.seqused_k) sk = cache_len(p, b);
+    int L = 0;                                             // TREE: cached rows in front of the drafted ones
+    if constexpr (TREE) {
+        L = tree_prefix(p.seqused_k, b, p.sk);
+        sk = (int)min((long long)L + sq, (long long)p.sk);
+    } else if (p.seqused_k) sk = cache_len(p, b);
     const int kb = p.cache_batch_idx ? p.cache_batch_idx[b] : b;
 
     const int rows_total = a.pack ? sq * G : sq;
@@ -57,7 +66,12 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
     // key range of this call (cross-device shard) and of this CTA (window, split)
     const int rb = max(0, p.kv_begin), re = p.kv_end > 0 ? min(sk, p.kv_end) : sk;
     int nb_lo = rb / BN, nb_hi = ceil_div(max(re, 0), BN);
-    {
+    if constexpr (TREE) {
+        int t_lo, t_hi;
+        tree_split_tiles(tree_first_any(a.tree, L), sk, a.nsplit, split, a.min_split_keys, t_lo, t_hi);
+        nb_lo = t_lo * (128 / BN);
+        nb_hi = min(t_hi * (128 / BN), ceil_div(sk, BN));
+    } else {
         const int qlo = a.pack ? m0 / G : m0;
         const int qhi = a.pack ? (min(rows_total, m0 + BM) - 1) / G : min(rows_total, m0 + BM) - 1;
         int lo, hi, lo2, hi2;
@@ -67,7 +81,7 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
         nb_hi = min(nb_hi, hi2 / BN + 1);
         if (hi2 < 0) nb_hi = nb_lo;
     }
-    if (a.nsplit > 1) {
+    if (!TREE && a.nsplit > 1) {
         const int s_lo = nb_lo + split * a.blocks_per_split;
         nb_hi = min(nb_hi, s_lo + a.blocks_per_split);
         nb_lo = s_lo;
@@ -75,6 +89,7 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
 
     // ---- per-thread row bookkeeping (two rows: g and g + 8 of the warp's 16) -----------
     int vrow[2], qpos[2], head[2], klo[2], khi[2];
+    const uint32_t* trow[2] = {a.tree.bits, a.tree.bits};
     float slope[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -82,12 +97,15 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
         const bool ok = vrow[r] < rows_total;
         qpos[r] = a.pack ? vrow[r] / G : vrow[r];
         head[r] = a.pack ? hk * G + vrow[r] % G : blockIdx.y;
-        if (ok) {
+        if (ok && TREE) {
+            klo[r] = tree_first_key(a.tree, b, qpos[r], L);
+            trow[r] = a.tree.bits + (int64_t)(b * a.tree.tokens + qpos[r]) * a.tree.words;
+        } else if (ok) {
             window_bounds(qpos[r], sq, sk, wl, wr, klo[r], khi[r]);
             klo[r] = max(klo[r], rb);
             khi[r] = min(khi[r], re - 1);
         } else {
-            klo[r] = 1; khi[r] = 0; head[r] = hk * G;
+            klo[r] = TREE ? 0x7fffffff : 1; khi[r] = 0; head[r] = hk * G;
         }
         slope[r] = p.alibi_slopes ? p.alibi_slopes[(int64_t)b * p.alibi_stride_b + head[r]] * kLog2e : 0.f;
     }
@@ -104,7 +122,8 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
         const bool ok = vr < rows_total && c * 8 < p.d;
         const int qp = a.pack ? vr / G : vr;
         const int hh = a.pack ? hk * G + vr % G : blockIdx.y;
-        const T* src = ok ? qbase + (int64_t)(q_off + qp) * p.q.stride_s + (int64_t)hh * p.q.stride_h + c * 8 : qbase;
+        const T* src = !ok ? qbase : TREE ? qbase + (int64_t)hk * p.q.stride_h + (int64_t)vr * p.q.stride_s + c * 8
+                                          : qbase + (int64_t)(q_off + qp) * p.q.stride_s + (int64_t)hh * p.q.stride_h + c * 8;
         cp_async16(smem_u32(sQ) + swz<PITCH>(r, c), src, ok ? 16 : 0);
     }
 
@@ -113,8 +132,14 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
         for (int idx = tid; idx < BN * CHUNKS; idx += 128) {
             const int r = idx / CHUNKS, c = idx % CHUNKS;
             const int tok = n0 + r;
-            const bool ok = tok < sk;
+            bool ok = tok < sk;
             int64_t koff = 0, voff = 0;
+            if constexpr (TREE) {
+                // rows of drafted tokens that are not there hold whatever was there before; a page that is not in the cache
+                // reads as zeros, as in the tile copies
+                if (ok && tok >= L) ok = (a.tree.keys[b * a.tree.words + ((tok - L) >> 5)] >> ((tok - L) & 31)) & 1;
+                if (ok) ok = (uint64_t)(int64_t)(btab ? btab[tok / p.page_size] : kb) < (uint64_t)p.kv_entries;
+            }
             if (ok) {
                 if (btab) {
                     const int blk = btab[tok / p.page_size];
@@ -181,6 +206,11 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             float mx = -INFINITY;
+            uint32_t vis[BN / 32] = {};
+            if constexpr (TREE) {
+#pragma unroll
+                for (int w = 0; w < BN / 32; ++w) vis[w] = klo[r] == 0x7fffffff ? 0u : tree_visible32(a.tree, trow[r], n0 + w * 32, klo[r], L);
+            }
 #pragma unroll
             for (int nt = 0; nt < BN / 8; ++nt) {
 #pragma unroll
@@ -189,7 +219,8 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
                     float x = s[nt][2 * r + e];
                     x = has_cap ? cap_out * tanhf(x * cap_in) : x * scale_log2;
                     if (p.alibi_slopes) x -= slope[r] * fabsf((float)(qpos[r] + sk - sq - col));
-                    x = (col >= klo[r] && col <= khi[r]) ? x : -INFINITY;
+                    if constexpr (TREE) x = (vis[nt / 4] >> ((nt & 3) * 8 + 2 * t + e)) & 1 ? x : -INFINITY;
+                    else x = (col >= klo[r] && col <= khi[r]) ? x : -INFINITY;
                     s[nt][2 * r + e] = x;
                     mx = fmaxf(mx, x);
                 }
@@ -296,12 +327,12 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
     }
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool TREE>
 static int launch_one(const FwdArgs& a, cudaStream_t st) {
     const fa_fwd_params& p = a.p;
     const int G = p.hq / p.hkv;
     const size_t smem = (size_t)(kGenericBM + 4 * kGenericBN) * HD * 2;
-    auto kern = fwd_generic_kernel<T, HD>;
+    auto kern = fwd_generic_kernel<T, HD, TREE>;
     static bool configured[16] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -319,8 +350,37 @@ static int launch_one(const FwdArgs& a, cudaStream_t st) {
     return cuda_ok(cudaGetLastError(), "fwd_generic launch");
 }
 
+template <bool TREE>
+static int launch_dims(const FwdArgs& a) {
+    const fa_fwd_params& p = a.p;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(p.stream);
+    const int dmax = p.d > p.dv ? p.d : p.dv;
+    note_kernel("generic_mma");
+    if (p.dtype == FA_F16) {
+        if (dmax <= 64) return launch_one<__half, 64, TREE>(a, st);
+        if (dmax <= 128) return launch_one<__half, 128, TREE>(a, st);
+        return launch_one<__half, 256, TREE>(a, st);
+    }
+    if (dmax <= 64) return launch_one<__nv_bfloat16, 64, TREE>(a, st);
+    if (dmax <= 128) return launch_one<__nv_bfloat16, 128, TREE>(a, st);
+    return launch_one<__nv_bfloat16, 256, TREE>(a, st);
+}
+
+int launch_fwd_generic_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, float* o_part, float* lse_part) {
+    FwdArgs a = {};
+    a.p = p;
+    a.nsplit = nsplit;
+    a.pack = 1;
+    a.o_part = o_part;
+    a.lse_part = lse_part;
+    a.part_minus_inf = o_part != nullptr;
+    a.tree = tree;
+    a.min_split_keys = min_split_keys;
+    return launch_dims<true>(a);
+}
+
 int launch_fwd_generic(const fa_fwd_params& p, const FwdPlan& plan, float* o_part, float* lse_part) {
-    FwdArgs a;
+    FwdArgs a = {};
     a.p = p;
     a.nsplit = plan.nsplit;
     a.blocks_per_split = plan.blocks_per_split;
@@ -328,17 +388,7 @@ int launch_fwd_generic(const fa_fwd_params& p, const FwdPlan& plan, float* o_par
     a.o_part = o_part;
     a.lse_part = lse_part;
     a.part_minus_inf = o_part != nullptr;
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(p.stream);
-    const int dmax = p.d > p.dv ? p.d : p.dv;
-    note_kernel("generic_mma");
-    if (p.dtype == FA_F16) {
-        if (dmax <= 64) return launch_one<__half, 64>(a, st);
-        if (dmax <= 128) return launch_one<__half, 128>(a, st);
-        return launch_one<__half, 256>(a, st);
-    }
-    if (dmax <= 64) return launch_one<__nv_bfloat16, 64>(a, st);
-    if (dmax <= 128) return launch_one<__nv_bfloat16, 128>(a, st);
-    return launch_one<__nv_bfloat16, 256>(a, st);
+    return launch_dims<false>(a);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -38,6 +38,14 @@ class FwdParams(C.Structure):
     ]
 
 
+class TreeParams(C.Structure):
+    _fields_ = [
+        ("fwd", FwdParams), ("parents", C.c_void_p), ("parents_stride_b", C.c_int64),
+        ("positions", C.c_void_p), ("positions_stride_axis", C.c_int64), ("positions_stride_b", C.c_int64),
+        ("axis_of_pair", C.c_void_p), ("axes", C.c_int32),
+    ]
+
+
 class BwdParams(C.Structure):
     _fields_ = [
         ("dout", FaTensor), ("q", FaTensor), ("k", FaTensor), ("v", FaTensor), ("o", FaTensor),
@@ -114,6 +122,8 @@ EXPORTS = {
     "fa_static_scratch_bytes": (C.c_size_t, []),
     "fa_fwd_workspace_bytes": (C.c_size_t, [C.POINTER(FwdParams)]),
     "fa_fwd_num_splits": (C.c_int, [C.POINTER(FwdParams)]),
+    "fa_tree_fwd_kvcache": (C.c_int, [C.POINTER(TreeParams)]),
+    "fa_tree_workspace_bytes": (C.c_size_t, [C.POINTER(TreeParams)]),
     "fa_bwd": (C.c_int, [C.POINTER(BwdParams)]),
     "fa_varlen_bwd": (C.c_int, [C.POINTER(BwdParams)]),
     "fa_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(BwdParams)]),
@@ -190,7 +200,7 @@ class Block:
         return buf
 
 
-FWD_BLOCK, BWD_BLOCK = Block(FwdParams), Block(BwdParams)
+FWD_BLOCK, BWD_BLOCK, TREE_BLOCK = Block(FwdParams), Block(BwdParams), Block(TreeParams)
 _POINTER = struct.Struct("=Q").pack_into
 
 
@@ -202,13 +212,14 @@ def _entry(name, restype):
 
 _call_fwd, _call_varlen_fwd, _call_kvcache = (_entry(n, C.c_int) for n in ("fa_fwd", "fa_varlen_fwd", "fa_fwd_kvcache"))
 _call_bwd, _call_varlen_bwd = (_entry(n, C.c_int) for n in ("fa_bwd", "fa_varlen_bwd"))
+_call_tree, _tree_bytes = _entry("fa_tree_fwd_kvcache", C.c_int), _entry("fa_tree_workspace_bytes", C.c_size_t)
 _fwd_bytes, _bwd_bytes, _bwd_min_bytes = (_entry(n, C.c_size_t) for n in (
     "fa_fwd_workspace_bytes", "fa_bwd_workspace_bytes", "fa_bwd_workspace_min_bytes"))
 
 
-def set_workspace(block, buf, ws, nbytes):
-    _POINTER(buf, block.offsets["workspace"], ws.data_ptr())
-    _POINTER(buf, block.offsets["workspace_bytes"], nbytes)
+def set_workspace(block, buf, ws, nbytes, prefix=""):
+    _POINTER(buf, block.offsets[prefix + "workspace"], ws.data_ptr())
+    _POINTER(buf, block.offsets[prefix + "workspace_bytes"], nbytes)
 
 
 if hasattr(torch._C, "_cuda_getCurrentRawStream"):

@@ -6,6 +6,7 @@ from .flash_attn_npu_interface import (  # noqa: F401
     flash_attn_func,
     flash_attn_mla_with_kvcache,
     flash_attn_qkvpacked_func,
+    flash_attn_tree_with_kvcache,
     flash_attn_varlen_func,
     flash_attn_with_kvcache,
     get_scheduler_metadata,

@@ -10,6 +10,7 @@ import torch
 import fa_b200_capi as capi
 from fa_b200_capi import CombineParams, SchedParams, check, lib, ptr
 from flash_attn_npu import flash_attn_npu as _v2
+from .rotary_axes import axis_pointer, check_positions
 
 
 def _reject(cond, what):
@@ -163,4 +164,116 @@ def mla_decode(q_nope, q_rope, latent_i8, scales, rope, block_table, cache_seqle
     p.stream = capi.stream_ptr(q_nope.device)
     with torch.cuda.device(q_nope.device):
         check(lib.fa_mla_decode(p))
+    return [out, lse]
+
+
+def _in_place(t):
+    """An input as 16-byte loads can read it: itself, or a copy where its last dim is strided or its rows are not aligned."""
+    s = t.stride()
+    return t if s[-1] == 1 and t.data_ptr() % 16 == 0 and not any(x % 8 for x in s[:-1]) else t.contiguous() if s[-1] != 1 else t.clone(
+        memory_format=torch.contiguous_format)
+
+
+def _int32(name, t, shapes, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise RuntimeError(f"{name} must be an int32 tensor")
+    if t.device != device:
+        raise RuntimeError(f"{name} must be on the device of q")
+    if tuple(t.shape) not in shapes:
+        raise RuntimeError(f"{name} must have shape " + " or ".join(str(s) for s in shapes))
+    return t if t.dim() == 0 or t.stride(-1) == 1 else t.contiguous()
+
+
+def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cache_batch_idx, page_table, rotary_cos, rotary_sin,
+                     rotary_positions, rotary_sections, rotary_sections_cyclic, rotary_interleaved, softmax_scale, window_size_left,
+                     window_size_right, softcap, num_splits):
+    """Attention of drafted tokens over a cache (no counterpart in the reference) -> [out, softmax_lse (B,H,T)]."""
+    capi.require_cuda(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cache_batch_idx, page_table, rotary_cos, rotary_sin,
+                      rotary_positions)
+    if q.dim() != 4 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise RuntimeError("q must be (batch, tokens, nheads, headdim), k_cache and v_cache of one shape with four dimensions")
+    batch, tokens, hq, d = q.shape
+    hkv, device = k_cache.shape[2], q.device
+    code = _v2._dtype_code(q)
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k", k), ("v", v)):
+        if t is not None and (t.dtype != q.dtype or t.device != device):
+            raise RuntimeError(f"{name} must have the dtype and the device of q")
+    if k_cache.shape[3] != d or d % 8 != 0 or d > 256:
+        raise RuntimeError("q and the cache must have the same head dimension, a multiple of 8 of at most 256")
+    if hkv == 0 or hq % hkv != 0:
+        raise RuntimeError("Number of heads in key/value must divide number of heads in query")
+    if k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
+        raise RuntimeError("k_cache and v_cache must have contiguous last dimension")
+    if (k is None) != (v is None):
+        raise RuntimeError("k and v must be passed together")
+    if k is not None and (tuple(k.shape) != (batch, tokens, hkv, d) or tuple(v.shape) != (batch, tokens, hkv, d)):
+        raise RuntimeError(f"k and v must have shape {(batch, tokens, hkv, d)}")
+    if window_size_right not in (-1, 0):
+        raise RuntimeError("a tree of tokens has no window to the right")
+    if softcap < 0.0:
+        raise RuntimeError("softcap must be non-negative (0.0 disables softcap)")
+    if num_splits < 0:
+        raise RuntimeError("num_splits must be >= 0")
+    cache_seqlens = _int32("cache_seqlens", cache_seqlens, [(batch,)], device)
+    tree_parents = _int32("tree_parents", tree_parents, [(batch, tokens), (tokens,)], device)
+    if page_table is not None:
+        if cache_batch_idx is not None:
+            raise RuntimeError("cache_batch_idx is not used with a paged cache")
+        page_table = _int32("page_table", page_table, [(batch, page_table.shape[-1])], device)
+        table, capacity = (page_table.data_ptr(), page_table.stride(0), k_cache.shape[1]), page_table.shape[1] * k_cache.shape[1]
+    else:
+        table, capacity = (0, 0, 0), k_cache.shape[1]
+        if cache_batch_idx is not None:
+            cache_batch_idx = _int32("cache_batch_idx", cache_batch_idx, [(batch,)], device)
+            cache_batch_idx = cache_batch_idx.contiguous()
+        elif k_cache.shape[0] < batch:
+            raise RuntimeError("the cache has fewer entries than the batch")
+    rotary, positions, axes = (0, 0, 0, 0, 0), (0, 0, 0), (0, 1)
+    keep = []
+    if rotary_cos is None:
+        if rotary_positions is not None or rotary_sections is not None:
+            raise RuntimeError("rotary positions and sections need rotary_cos and rotary_sin")
+    else:
+        if k is None:
+            raise RuntimeError("rotary embedding is only applied when k and v are passed in")
+        if rotary_sin is None or rotary_cos.dim() != 2 or rotary_cos.shape != rotary_sin.shape:
+            raise RuntimeError("rotary_cos and rotary_sin must both have shape (seqlen_ro, rotary_dim / 2)")
+        if rotary_cos.device != device or rotary_sin.device != device:
+            raise RuntimeError("rotary_cos and rotary_sin must be on the device of q")
+        pairs = rotary_cos.shape[1]
+        if rotary_cos.shape[0] == 0 or not 0 < 2 * pairs <= d:
+            raise RuntimeError("rotary_dim must be positive and at most the head dimension, with one table row at least")
+        rc, rs = rotary_cos.to(q.dtype).contiguous(), rotary_sin.to(q.dtype).contiguous()
+        rotary = (rc.data_ptr(), rs.data_ptr(), 2 * pairs, int(rotary_interleaved), rc.shape[0])
+        axis, where, n = axis_pointer(pairs, rotary_sections, rotary_sections_cyclic)
+        axes = (where, n)
+        keep += [rc, rs, axis]
+        if rotary_positions is not None:
+            pos = check_positions(rotary_positions, n, (batch, tokens), device)
+            pos = pos if pos.stride(-1) == 1 else pos.contiguous()
+            positions = (pos.data_ptr(), pos.stride(0), pos.stride(1))
+            keep.append(pos)
+    out = torch.empty((batch, tokens, hq, d), dtype=q.dtype, device=device)
+    lse = torch.empty((batch, hq, tokens), dtype=torch.float32, device=device)
+    if batch == 0 or tokens == 0:
+        return [out, lse]
+    if k_cache.numel() == 0:
+        raise RuntimeError("the cache has no rows")
+    q = _in_place(q)
+    new = _v2._NO_TENSOR + _v2._NO_TENSOR
+    if k is not None:
+        k, v = _in_place(k), _in_place(v)
+        new = _v2._leaves(k) + _v2._leaves(v)
+    parents_sb = tree_parents.stride(0) if tree_parents.dim() == 2 else 0
+    buf = capi.TREE_BLOCK.new(
+        *_v2._leaves(q), *_v2._leaves(k_cache), *_v2._leaves(v_cache), *_v2._leaves(out), lse.data_ptr(), *lse.stride(),
+        0, 0, cache_seqlens.data_ptr(), *table, 0 if cache_batch_idx is None else cache_batch_idx.data_ptr(), 0, 0,
+        batch, tokens, capacity, 0, 0, hq, hkv, d, d, softmax_scale, softcap, 0, _v2._i32(window_size_left), -1, code,
+        *new, tokens, *rotary, num_splits, 0, 0, 0, 0, 0, 0, 0, 0, k_cache.shape[0], capi.raw_stream(device),
+        tree_parents.data_ptr(), parents_sb, *positions, *axes)
+    nbytes = capi._tree_bytes(buf)
+    ws = capi.workspace(nbytes, device)
+    capi.set_workspace(capi.TREE_BLOCK, buf, ws, nbytes, "fwd.")
+    capi.launch(capi._call_tree, buf, device)
+    del keep
     return [out, lse]

@@ -364,3 +364,40 @@ def flash_attn_mla_with_kvcache(q_nope, q_rope, latent_cache_i8, latent_scales, 
     out, lse = _ext.mla_decode(q_nope, q_rope, latent_cache_i8, latent_scales, rope_cache, page_table, cache_seqlens,
                                softmax_scale, num_splits)
     return (out, lse) if return_softmax_lse else out
+
+
+def flash_attn_tree_with_kvcache(q, k_cache, v_cache, k, v, tree_parents,
+                                 cache_seqlens: Union[int, torch.Tensor] = None,
+                                 cache_batch_idx: Optional[torch.Tensor] = None,
+                                 page_table: Optional[torch.Tensor] = None, rotary_cos=None, rotary_sin=None,
+                                 rotary_positions: Optional[torch.Tensor] = None, rotary_sections=None,
+                                 rotary_sections_cyclic=False, rotary_interleaved=True, softmax_scale=None,
+                                 window_size=(-1, -1), softcap=0.0, num_splits=0, return_softmax_lse=False):
+    """Attention of a tree of drafted tokens over a KV cache, for speculative decoding with several continuations at once
+    (no backward; an addition of this library).
+
+    q (batch, tokens, nheads, headdim) with at most 256 tokens; k_cache / v_cache dense (batch_cache, seqlen_cache, nheads_k,
+    headdim) or paged (num_pages, page_size, nheads_k, headdim) with an int32 page_table (batch, max_pages), as in
+    flash_attn_with_kvcache.  cache_seqlens (int or int32 (batch,)): the rows in front of the draft.  k, v (batch, tokens,
+    nheads_k, headdim) are written into the cache IN PLACE at rows cache_seqlens .. cache_seqlens + tokens - 1; None when they
+    stand there already.
+
+    tree_parents (batch, tokens), or (tokens,) for all sequences, int32: the parent of each token, a token in front of it, or
+    -1 for a child of the last cached row.  A token attends to all cached rows, its ancestors and itself.  Any other value,
+    such as the -2 of a padded draft, says that there is no token: nothing is written, nobody sees it, its output is zero and
+    its softmax_lse +inf; a child of such a token is none either.  V of the tokens that are there must be finite: a tile's
+    masked probabilities are exact zeros, and 0 x NaN is NaN.
+
+    Position of a token: cache_seqlens + its depth.  window_size = (left, -1) keeps keys at most `left` positions back.
+    rotary_cos / rotary_sin (seqlen_ro, rotary_dim / 2), taken in q's dtype, turn q and k by the row of that position, or by
+    rotary_positions (axes, batch, tokens) int32 with rotary_sections = pairs of each axis (see rotary_axes_func).  A position
+    outside the tables takes the nearest row.  Rows past the cache's capacity, or on a page that is not in the cache, are
+    neither written nor seen.  Returns out (batch, tokens, nheads, headdim), or (out, softmax_lse (batch, nheads, tokens))."""
+    if softmax_scale is None:
+        softmax_scale = q.shape[-1] ** (-0.5)
+    if isinstance(cache_seqlens, int):
+        cache_seqlens = torch.full((q.shape[0],), cache_seqlens, dtype=torch.int32, device=q.device)
+    out, lse = _ext.tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cache_batch_idx, page_table, rotary_cos,
+                                     rotary_sin, rotary_positions, rotary_sections, rotary_sections_cyclic, rotary_interleaved,
+                                     softmax_scale, window_size[0], window_size[1], softcap, num_splits)
+    return (out, lse) if return_softmax_lse else out

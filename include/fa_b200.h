@@ -131,6 +131,39 @@ size_t fa_fwd_workspace_bytes(const fa_fwd_params* p);
 int    fa_fwd_num_splits(const fa_fwd_params* p);
 
 /* ------------------------------------------------------------------------
+ * Attention of a tree of drafted tokens over a KV cache (speculative decoding
+ * with several continuations).  No counterpart in the reference, whose cache
+ * calls (mha_fwd_kvcache, flash_api.cpp:356) know causal and windowed masks.
+ * `fwd` is filled as for fa_fwd_kvcache: q (b, sq tokens, hq, d), the cache,
+ * seqused_k = cached rows L in front of the draft, k_new / v_new (written to
+ * rows L .. L + sq - 1; null when they stand there already), rotary, window_left,
+ * softcap, num_splits, kv_entries (required), workspace of
+ * fa_tree_workspace_bytes().  Not used: causal, window_right, alibi, cu_seqlens,
+ * kv_begin / kv_end, partials, sched_meta.  d == dv, at most 256 tokens.
+ * Token t sees the cached rows, itself and its ancestors.  parents[t] is a token
+ * in front of t, or -1 for a child of the last cached row; any other value (and
+ * a child of such a token) is no token: nothing is written for it, nobody sees
+ * it, its output is 0 and its LSE +inf.  A window of window_left counts positions
+ * L + depth.  Rows of the draft that lie past the capacity, or on a page that is
+ * not in the cache, are neither written nor seen; a cached row on such a page
+ * reads as zeros.
+ * Rotary turns pair i of q and k_new by table row positions[axis_of_pair[i]][b][t],
+ * or by row L + depth(t) where positions is null.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    fa_fwd_params  fwd;
+    const int32_t* parents;               /* (b, sq) on the device                           */
+    int64_t        parents_stride_b;      /* 0 when all sequences have the same tree          */
+    const int32_t* positions;             /* (axes, b, sq) on the device, or null             */
+    int64_t        positions_stride_axis, positions_stride_b;
+    const uint8_t* axis_of_pair;          /* HOST, rotary_dim / 2 bytes, or null = axis 0     */
+    int32_t        axes;                  /* 1 .. 4                                          */
+} fa_tree_params;
+
+int    fa_tree_fwd_kvcache(const fa_tree_params* p);
+size_t fa_tree_workspace_bytes(const fa_tree_params* p);
+
+/* ------------------------------------------------------------------------
  * Backward.   fa_bwd: mha_bwd flash_api.cpp:1279 (launch_fag_general,
  * fag_general_host.cpp:18);  fa_varlen_bwd: mha_varlen_bwd flash_api.cpp:1092;
  * v3 mha_bwd csrc/ascend910/flash_attn_npu_3/flash_api.cpp:573.
