@@ -1,0 +1,180 @@
+// Rotary embedding of q and k with one to four position axes, forward and backward (rotary_axes.cuh has the formula; the
+// backward turns by the negative angle).  The reference only rotates inside its cache call (flash_attn_npu_interface.py:1469),
+// by one position a token.
+//
+// Bound by HBM: (Hq + Hkv) D elements a token are read and written once, 4 bytes each way together.  One launch does q and k,
+// so that the tables and positions are looked up once a token: a thread keeps the eight cosines and sines of its unit (two
+// 16-byte chunks that hold each other's partners) in registers and walks over heads.
+#include <cstring>
+#include "fa_utils.cuh"
+#include "fa_internal.h"
+#include "rotary_axes.cuh"
+
+namespace fa {
+
+namespace {
+
+struct RotaryArgs {
+    RotaryAxes ro;
+    fa_tensor src[2], dst[2];        // q, k
+    int heads[2];                    // heads of k: 0 = no k
+    int d, units, tokens, batch;     // units: ceil(d / 16) of a head's row
+    int lanes_h, iters;              // heads side by side in a CTA's row of threads, heads one after the other in a thread
+    int in_place;                    // columns behind the rotated ones stay where they are
+    float sign;                      // -1: turn back
+};
+
+constexpr int kThreads = 128;
+
+// thread -> (unit, head lane) of a token; blockIdx.x: token x group of heads
+template <typename T, typename TT, bool VEC>
+__global__ void __launch_bounds__(kThreads) rotary_axes_kernel(const __grid_constant__ RotaryArgs a) {
+    const int heads = a.heads[0] + a.heads[1];
+    const int groups = (heads + a.lanes_h * a.iters - 1) / (a.lanes_h * a.iters);
+    const int64_t slot = (int64_t)blockIdx.x * (kThreads / (a.units * a.lanes_h)) + threadIdx.x / (a.units * a.lanes_h);
+    if (threadIdx.x >= kThreads / (a.units * a.lanes_h) * (a.units * a.lanes_h)) return;
+    const int64_t token = slot / groups;
+    if (token >= (int64_t)a.batch * a.tokens) return;
+    const int group = (int)(slot % groups);
+    const int in_slot = threadIdx.x % (a.units * a.lanes_h);
+    const int u = in_slot % a.units, hl = in_slot / a.units;
+    const int b = (int)(token / a.tokens), t = (int)(token % a.tokens);
+    const RotaryRows rows = rotary_rows(a.ro, b, t);
+    const bool turned = u < (a.ro.rd + 15) / 16;
+    if (!turned && a.in_place) return;
+    float c[8], s[8];
+    int lo = 2 * u, hi = 2 * u + 1;
+    if (VEC && turned) {
+        unit_chunks(a.ro, u, lo, hi);
+        load_angles8<TT>(a.ro, rows, u * 8, c, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] *= a.sign;
+    }
+    const bool two = hi < a.d / 8;
+    const int h0 = group * a.lanes_h * a.iters + hl;
+    auto row_of = [&](int h, const T*& src, T*& dst) {
+        const int w = h >= a.heads[0];
+        const int hh = w ? h - a.heads[0] : h;
+        const fa_tensor &x = a.src[w], &y = a.dst[w];
+        src = reinterpret_cast<const T*>(x.ptr) + (int64_t)b * x.stride_b + (int64_t)t * x.stride_s + (int64_t)hh * x.stride_h;
+        dst = reinterpret_cast<T*>(y.ptr) + (int64_t)b * y.stride_b + (int64_t)t * y.stride_s + (int64_t)hh * y.stride_h;
+    };
+    if constexpr (VEC) {
+        constexpr int N = 4;                                 // heads in flight
+        for (int i = 0; i < a.iters; i += N) {
+            uint4 xa[N], xb[N];
+            T* out[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int h = h0 + (i + k) * a.lanes_h;
+                out[k] = nullptr;
+                if (i + k < a.iters && h < heads) {
+                    const T* src;
+                    row_of(h, src, out[k]);
+                    xa[k] = reinterpret_cast<const uint4*>(src)[lo];
+                    if (two) xb[k] = reinterpret_cast<const uint4*>(src)[hi];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                if (!out[k]) continue;
+                uint4 ya = xa[k], yb = xb[k];
+                if (turned) turn8<T>(xa[k], xb[k], c, s, a.ro.interleaved, ya, yb);
+                reinterpret_cast<uint4*>(out[k])[lo] = ya;
+                if (two) reinterpret_cast<uint4*>(out[k])[hi] = yb;
+            }
+        }
+    } else {
+        // element by element; in place every pair is written by the thread that read it: units of 8 pairs, then the rest
+        for (int i = 0; i < a.iters; ++i) {
+            const int h = h0 + i * a.lanes_h;
+            if (h >= heads) break;
+            const T* src;
+            T* dst;
+            row_of(h, src, dst);
+            const int pairs = a.ro.rd / 2;
+            for (int k = u * 8; k < min(u * 8 + 8, pairs); ++k) {
+                const int e = a.ro.interleaved ? 2 * k : k, f = a.ro.interleaved ? 2 * k + 1 : k + pairs;
+                const T ye = turn_elem<T, TT>(src, e, a.ro, rows, a.sign), yf = turn_elem<T, TT>(src, f, a.ro, rows, a.sign);
+                dst[e] = ye;
+                dst[f] = yf;
+            }
+            if (!a.in_place)
+                for (int e = max(a.ro.rd, u * 16); e < min(a.d, u * 16 + 16); ++e) dst[e] = src[e];
+        }
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T, typename TT>
+int launch(const RotaryArgs& a, bool vec, int64_t blocks, cudaStream_t st) {
+    if (vec) rotary_axes_kernel<T, TT, true><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+    else rotary_axes_kernel<T, TT, false><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+    mark_kernel(st);
+    return cuda_ok(cudaGetLastError(), "rotary_axes launch");
+}
+
+int run_rotary(const fa_rotary_params& r) {
+    if (r.dtype != FA_F16 && r.dtype != FA_BF16) return fail(FA_ERR_BAD_DTYPE, "only fp16 and bf16 are supported");
+    if (r.table_dtype != r.dtype && r.table_dtype != 2) return fail(FA_ERR_BAD_DTYPE, "the tables must have the dtype of q or fp32");
+    if (r.b < 0 || r.s < 0 || r.hq < 0 || r.hk < 0 || r.hq + r.hk <= 0) return fail(FA_ERR_BAD_SHAPE, "negative or zero size");
+    if (r.d <= 0 || r.d > 256 || r.d % 2) return fail(FA_ERR_BAD_SHAPE, "head dimension must be even and at most 256");
+    if (r.rotary_dim <= 0 || r.rotary_dim > r.d || r.rotary_dim % 2) return fail(FA_ERR_BAD_SHAPE, "rotary_dim must be even and <= headdim");
+    if (r.seqlen_ro <= 0) return fail(FA_ERR_BAD_SHAPE, "seqlen_ro must be positive");
+    if (r.axes < 1 || r.axes > kMaxAxes) return fail(FA_ERR_BAD_SHAPE, "one to four position axes");
+    if (!r.cos || !r.sin || !r.positions) return fail(FA_ERR_NULL, "cos, sin or positions is null");
+    if (r.hq && (!r.q.ptr || !r.q_out.ptr)) return fail(FA_ERR_NULL, "q is null");
+    if (r.hk && (!r.k.ptr || !r.k_out.ptr)) return fail(FA_ERR_NULL, "k is null");
+    if (r.b == 0 || r.s == 0) return FA_OK;
+    RotaryArgs a = {};
+    a.ro.cos = r.cos;
+    a.ro.sin = r.sin;
+    a.ro.positions = r.positions;
+    a.ro.pos_stride_axis = r.positions_stride_axis;
+    a.ro.pos_stride_b = r.positions_stride_b;
+    a.ro.rd = r.rotary_dim;
+    a.ro.interleaved = r.interleaved;
+    a.ro.rows = r.seqlen_ro;
+    a.ro.axes = r.axes;
+    pack_axes(a.ro, r.axis_of_pair);
+    a.src[0] = r.q; a.dst[0] = r.q_out;
+    a.src[1] = r.k; a.dst[1] = r.k_out;
+    a.heads[0] = r.hq; a.heads[1] = r.hk;
+    a.d = r.d;
+    a.units = (r.d + 15) / 16;
+    a.batch = r.b; a.tokens = r.s;
+    a.sign = r.backward ? -1.f : 1.f;
+    a.in_place = (!r.hq || r.q.ptr == r.q_out.ptr) && (!r.hk || r.k.ptr == r.k_out.ptr);
+    const int heads = r.hq + r.hk;
+    int side = kThreads / a.units;
+    a.lanes_h = 1;
+    while (a.lanes_h * 2 <= side && a.lanes_h < 4 && a.lanes_h < heads) a.lanes_h *= 2;
+    const int per = (heads + a.lanes_h - 1) / a.lanes_h;     // heads of a thread if a token is one slot
+    const int64_t tokens = (int64_t)r.b * r.s;
+    // few tokens: their heads are spread over more threads, until every SM has something to do
+    int groups = 1;
+    while (groups * 2 <= per && tokens * groups * a.units * a.lanes_h < (int64_t)sm_count() * 512) groups *= 2;
+    a.iters = (per + groups - 1) / groups;
+    groups = (per + a.iters - 1) / a.iters;
+    const int slots = kThreads / (a.units * a.lanes_h);
+    const int64_t blocks = (tokens * groups + slots - 1) / slots;
+    if (blocks >= (1ll << 31)) return fail(FA_ERR_BAD_SHAPE, "too many tokens");
+    bool vec = r.rotary_dim % 16 == 0 && r.d % 8 == 0 && aligned16(r.cos) && aligned16(r.sin);
+    const fa_tensor* ts[4] = {&a.src[0], &a.dst[0], &a.src[1], &a.dst[1]};
+    for (int i = r.hq ? 0 : 2; i < (r.hk ? 4 : 2); ++i)
+        vec = vec && aligned16(ts[i]->ptr) && (ts[i]->stride_b | ts[i]->stride_s | ts[i]->stride_h) % 8 == 0;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(r.stream);
+    mark_kernel(st);
+    if (r.dtype == FA_F16)
+        return r.table_dtype == 2 ? launch<__half, float>(a, vec, blocks, st) : launch<__half, __half>(a, vec, blocks, st);
+    return r.table_dtype == 2 ? launch<__nv_bfloat16, float>(a, vec, blocks, st) : launch<__nv_bfloat16, __nv_bfloat16>(a, vec, blocks, st);
+}
+
+}  // namespace
+}  // namespace fa
+
+extern "C" int fa_rotary_axes(const fa_rotary_params* r) {
+    if (!r) return fa::fail(FA_ERR_NULL, "params is null");
+    return fa::run_rotary(*r);
+}

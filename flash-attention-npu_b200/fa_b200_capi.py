@@ -46,6 +46,17 @@ class TreeParams(C.Structure):
     ]
 
 
+class RotaryParams(C.Structure):
+    _fields_ = [
+        ("q", FaTensor), ("k", FaTensor), ("q_out", FaTensor), ("k_out", FaTensor),
+        ("cos", C.c_void_p), ("sin", C.c_void_p),
+        ("positions", C.c_void_p), ("positions_stride_axis", C.c_int64), ("positions_stride_b", C.c_int64),
+        ("axis_of_pair", C.c_void_p), ("axes", C.c_int32), ("b", C.c_int32), ("s", C.c_int32), ("hq", C.c_int32), ("hk", C.c_int32),
+        ("d", C.c_int32), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("seqlen_ro", C.c_int32), ("backward", C.c_int32),
+        ("dtype", C.c_int32), ("table_dtype", C.c_int32), ("stream", C.c_void_p),
+    ]
+
+
 class BwdParams(C.Structure):
     _fields_ = [
         ("dout", FaTensor), ("q", FaTensor), ("k", FaTensor), ("v", FaTensor), ("o", FaTensor),
@@ -114,6 +125,24 @@ class SchedParams(C.Structure):
     ]
 
 
+class CacheView(C.Structure):
+    _fields_ = [
+        ("ptr", C.c_void_p), ("stride_cache", C.c_int64), ("stride_page", C.c_int64), ("stride_row", C.c_int64), ("stride_head", C.c_int64),
+        ("caches", C.c_int32), ("heads", C.c_int32), ("segment_bytes", C.c_int32),
+    ]
+
+
+class PagesParams(C.Structure):
+    _fields_ = [
+        ("caches", C.c_void_p), ("num_caches", C.c_int32), ("num_pages", C.c_int32), ("page_size", C.c_int32),
+        ("refs", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64),
+        ("b", C.c_int32), ("width", C.c_int32), ("extra", C.c_int32), ("n", C.c_int32), ("keep_parents", C.c_int32),
+        ("seqlens", C.c_void_p), ("rows", C.c_void_p), ("rows2", C.c_void_p), ("rows_stride", C.c_int64), ("cache_batch_idx", C.c_void_p),
+        ("new_table", C.c_void_p), ("new_seqlens", C.c_void_p), ("missing", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("stream", C.c_void_p),
+    ]
+
+
 EXPORTS = {
     "fa_fwd": (C.c_int, [C.POINTER(FwdParams)]),
     "fa_varlen_fwd": (C.c_int, [C.POINTER(FwdParams)]),
@@ -124,6 +153,13 @@ EXPORTS = {
     "fa_fwd_num_splits": (C.c_int, [C.POINTER(FwdParams)]),
     "fa_tree_fwd_kvcache": (C.c_int, [C.POINTER(TreeParams)]),
     "fa_tree_workspace_bytes": (C.c_size_t, [C.POINTER(TreeParams)]),
+    "fa_pages_reserve": (C.c_int, [C.POINTER(PagesParams)]),
+    "fa_pages_free": (C.c_int, [C.POINTER(PagesParams)]),
+    "fa_pages_fork": (C.c_int, [C.POINTER(PagesParams)]),
+    "fa_pages_copy": (C.c_int, [C.POINTER(PagesParams)]),
+    "fa_cache_compact": (C.c_int, [C.POINTER(PagesParams)]),
+    "fa_pages_workspace_bytes": (C.c_size_t, [C.c_int32, C.c_int32]),
+    "fa_rotary_axes": (C.c_int, [C.POINTER(RotaryParams)]),
     "fa_bwd": (C.c_int, [C.POINTER(BwdParams)]),
     "fa_varlen_bwd": (C.c_int, [C.POINTER(BwdParams)]),
     "fa_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(BwdParams)]),
@@ -201,6 +237,7 @@ class Block:
 
 
 FWD_BLOCK, BWD_BLOCK, TREE_BLOCK = Block(FwdParams), Block(BwdParams), Block(TreeParams)
+ROTARY_BLOCK, PAGES_BLOCK = Block(RotaryParams), Block(PagesParams)
 _POINTER = struct.Struct("=Q").pack_into
 
 
@@ -212,6 +249,9 @@ def _entry(name, restype):
 
 _call_fwd, _call_varlen_fwd, _call_kvcache = (_entry(n, C.c_int) for n in ("fa_fwd", "fa_varlen_fwd", "fa_fwd_kvcache"))
 _call_bwd, _call_varlen_bwd = (_entry(n, C.c_int) for n in ("fa_bwd", "fa_varlen_bwd"))
+_call_rotary = _entry("fa_rotary_axes", C.c_int)
+_call_reserve, _call_free, _call_fork, _call_copy, _call_compact = (_entry(n, C.c_int) for n in (
+    "fa_pages_reserve", "fa_pages_free", "fa_pages_fork", "fa_pages_copy", "fa_cache_compact"))
 _call_tree, _tree_bytes = _entry("fa_tree_fwd_kvcache", C.c_int), _entry("fa_tree_workspace_bytes", C.c_size_t)
 _fwd_bytes, _bwd_bytes, _bwd_min_bytes = (_entry(n, C.c_size_t) for n in (
     "fa_fwd_workspace_bytes", "fa_bwd_workspace_bytes", "fa_bwd_workspace_min_bytes"))

@@ -11,3 +11,11 @@ from .flash_attn_npu_interface import (  # noqa: F401
     flash_attn_with_kvcache,
     get_scheduler_metadata,
 )
+from .rotary_axes import rotary_axes_func  # noqa: F401
+from .kvcache_pages import (  # noqa: F401
+    kvcache_compact,
+    kvcache_copy_pages,
+    kvcache_fork,
+    kvcache_free,
+    kvcache_reserve,
+)

@@ -1,8 +1,12 @@
-"""Rotary position axes: which axis (time, height, width, ..) turns which pair of a head."""
+"""Rotary embedding with several position axes (an addition of this library; the reference rotates inside its cache call only,
+flash_attn_npu_3/flash_attn_npu_interface.py:965)."""
 import ctypes
 import functools
+from typing import List, Optional, Tuple
 
 import torch
+
+import fa_b200_capi as capi
 
 MAX_AXES = 4
 
@@ -39,8 +43,141 @@ def check_positions(positions, axes, lead, device):
         raise RuntimeError("positions must be an int32 tensor")
     if positions.device != device:
         raise RuntimeError("positions must be on the device of the tensors that they belong to")
-    if axes == 1 and tuple(positions.shape) == tuple(lead):
+    shape = tuple(positions.shape)
+    if axes == 1 and shape == lead:
         positions = positions.unsqueeze(0)
-    if tuple(positions.shape) != (axes, *lead):
-        raise RuntimeError(f"positions must have shape {(axes, *lead)}" + (f" or {tuple(lead)}" if axes == 1 else ""))
-    return positions
+    elif shape != (axes, *lead):
+        raise RuntimeError(f"positions must have shape {(axes, *lead)}" + (f" or {lead}" if axes == 1 else ""))
+    return positions if positions.stride(-1) == 1 or positions.shape[-1] == 1 else positions.contiguous()
+
+
+_NONE = (0, 0, 0, 0)
+
+
+def _leaves(t):
+    """The four leaves of an fa_tensor of (B, S, H, D), or of packed (T, H, D) as one batch entry."""
+    s = t.stride()
+    return (t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (t.data_ptr(), 0, s[0], s[1])
+
+
+def _run(q, k, q_out, k_out, cos, sin, positions, sections, cyclic, interleaved, backward):
+    """The library call; everything has been checked, positions is (axes, *lead)."""
+    pairs = cos.shape[1]
+    keep, axis, axes = axis_pointer(pairs, sections, cyclic)
+    packed = q.dim() == 3
+    b, s = (1, q.shape[0]) if packed else q.shape[:2]
+    pos = positions.stride()
+    d = q.shape[-1]
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        return
+    buf = capi.ROTARY_BLOCK.new(
+        *_leaves(q), *(_NONE if k is None else _leaves(k)), *_leaves(q_out), *(_NONE if k is None else _leaves(k_out)),
+        cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), pos[0], 0 if packed else pos[1], axis, axes, b, s,
+        q.shape[-2], 0 if k is None else k.shape[-2], d, 2 * pairs, int(interleaved), cos.shape[0], int(backward),
+        capi.DTYPES[q.dtype], 2 if cos.dtype == torch.float32 else capi.DTYPES[cos.dtype], capi.raw_stream(q.device))
+    capi.launch(capi._call_rotary, buf, q.device)
+    del keep
+
+
+def _out_of_place(q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
+    q, k = (x.contiguous() if x is not None and x.stride(-1) != 1 else x for x in (q, k))
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _run(q, k, q_out, k_out, cos, sin, positions, sections, cyclic, interleaved, backward)
+    return q_out, k_out
+
+
+@torch.library.custom_op("flash_attn_npu_3::_rotary_axes", mutates_args=(), device_types="cuda")
+def _rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                 sections: Optional[List[int]], cyclic: bool, interleaved: bool, backward: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    q_out, k_out = _out_of_place(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
+    return q_out, torch.empty((0,), dtype=q.dtype, device=q.device) if k is None else k_out
+
+
+@torch.library.register_fake("flash_attn_npu_3::_rotary_axes")
+def _rotary_axes_fake(q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
+    return q.new_empty(q.shape), q.new_empty((0,)) if k is None else k.new_empty(k.shape)
+
+
+def _forward(q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
+    if capi.plain(q, k, cos, sin, positions):                  # the op's dispatch would do nothing but call the body
+        return _out_of_place(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
+    q_out, k_out = _rotary_axes(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
+    return q_out, None if k is None else k_out
+
+
+class RotaryAxesFunc(torch.autograd.Function):
+    """A rotation is linear and orthogonal: its gradient is the rotation back, which is differentiable in the same way."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(cos, sin, positions)
+        ctx.args = (sections, cyclic, interleaved)
+        ctx.turn_back = not backward
+        return _forward(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        cos, sin, positions = ctx.saved_tensors
+        args = (cos, sin, positions, *ctx.args, ctx.turn_back)
+        if dq is not None and dk is not None:
+            dq, dk = _apply(dq, dk, *args)
+        elif dq is not None:
+            dq, _ = _apply(dq, None, *args)
+        elif dk is not None:
+            dk, _ = _apply(dk, None, *args)
+        return (dq, dk) + (None,) * 7
+
+
+def _apply(q, k, *args):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return RotaryAxesFunc.apply(q, k, *args)
+    return _forward(q, k, *args)
+
+
+def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=False, interleaved=False, inplace=False):
+    """Rotary embedding of q and k with one to four position axes (time, height, width, ..), differentiable in q and k.
+
+    q (batch, seqlen, nheads, headdim) or packed (total, nheads, headdim), fp16 or bf16; k of the same shape but for its heads,
+    or None.  cos / sin (seqlen_ro, rotary_dim / 2) in q's dtype or fp32.  positions int32 (axes, batch, seqlen) or
+    (axes, total); without the first dimension for one axis.  Pair i of a head - elements i and i + rotary_dim / 2, or 2 i and
+    2 i + 1 when interleaved - is turned by row positions[axis of i] of the tables, column i; columns behind rotary_dim are
+    copied.  sections: how many of the rotary_dim / 2 pairs each axis has, in consecutive blocks, or with sections_cyclic pair
+    i belongs to axis i % axes while that axis has pairs left, else to axis 0.  None: one axis.  A position outside the tables
+    takes the nearest row.  fp32 arithmetic, rounded once; cos, sin and positions get no gradient.
+
+    inplace writes into q and k instead of new tensors (only where no gradient is needed).
+    Returns (q, k), or q alone when k is None."""
+    capi.require_cuda(q, k, cos, sin, positions)
+    if q.dtype not in capi.DTYPES or (k is not None and k.dtype != q.dtype):
+        raise RuntimeError("rotary embedding only supports FP16 and BF16 data types, the same for q and k")
+    if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
+        raise RuntimeError("q must be (batch, seqlen, nheads, headdim) or (total, nheads, headdim), and k the same but for its heads")
+    device = q.device
+    if any(t is not None and t.device != device for t in (k, cos, sin)):
+        raise RuntimeError("q, k, cos and sin must be on one device")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.dtype not in (q.dtype, torch.float32):
+        raise RuntimeError("cos and sin must both have shape (seqlen_ro, rotary_dim / 2), in q's dtype or fp32")
+    d, pairs = q.shape[-1], cos.shape[1]
+    if d > 256 or d % 2 or not 0 < 2 * pairs <= d or cos.shape[0] == 0:
+        raise RuntimeError("the head dimension must be even and at most 256, rotary_dim positive and at most that, with one table row at least")
+    if sections is not None:
+        sections = list(sections)
+        axis_table(pairs, tuple(sections), bool(sections_cyclic))
+    positions = check_positions(positions, 1 if sections is None else len(sections), tuple(q.shape[:-2]), device)
+    if not cos.is_contiguous() or not sin.is_contiguous():
+        cos, sin = cos.contiguous(), sin.contiguous()
+    args = (cos, sin, positions, sections, bool(sections_cyclic), bool(interleaved))
+    if inplace:
+        for t in (q, k):
+            if t is None:
+                continue
+            if torch.is_grad_enabled() and t.requires_grad:
+                raise RuntimeError("inplace rotary embedding is not differentiable: detach q and k, or leave inplace out")
+            if t.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+                raise RuntimeError("inplace rotary embedding needs a contiguous last dimension and no expanded dimensions")
+        _run(q, k, q, k, *args, False)
+    else:
+        q, k = _apply(q, k, *args, False)
+    return q if k is None else (q, k)

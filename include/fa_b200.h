@@ -164,6 +164,29 @@ int    fa_tree_fwd_kvcache(const fa_tree_params* p);
 size_t fa_tree_workspace_bytes(const fa_tree_params* p);
 
 /* ------------------------------------------------------------------------
+ * Rotary embedding of q and k with one to four position axes (time, height,
+ * width, ..), out of place or in place (q_out.ptr == q.ptr); backward != 0 turns
+ * by the negative angle, which is the gradient.  Pair i of a head (elements i and
+ * i + rotary_dim / 2, or 2 i and 2 i + 1 when interleaved) is turned by table row
+ * positions[axis_of_pair[i]][b][s]; columns behind rotary_dim are copied.  A
+ * position outside the tables takes the nearest row.  No counterpart in the
+ * reference (it rotates inside its cache call, flash_attn_npu_interface.py:1469).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    fa_tensor q, k, q_out, k_out;         /* (b, s, heads, d); hq or hk = 0 leaves one out     */
+    const void*    cos;                   /* (seqlen_ro, rotary_dim / 2)                       */
+    const void*    sin;
+    const int32_t* positions;             /* (axes, b, s) on the device                        */
+    int64_t        positions_stride_axis, positions_stride_b;
+    const uint8_t* axis_of_pair;          /* HOST, rotary_dim / 2 bytes, or null = axis 0      */
+    int32_t axes, b, s, hq, hk, d, rotary_dim, interleaved, seqlen_ro, backward;
+    int32_t dtype, table_dtype;           /* fa_dtype; of the tables: the same, or 2 = fp32    */
+    void*   stream;
+} fa_rotary_params;
+
+int fa_rotary_axes(const fa_rotary_params* p);
+
+/* ------------------------------------------------------------------------
  * Backward.   fa_bwd: mha_bwd flash_api.cpp:1279 (launch_fag_general,
  * fag_general_host.cpp:18);  fa_varlen_bwd: mha_varlen_bwd flash_api.cpp:1092;
  * v3 mha_bwd csrc/ascend910/flash_attn_npu_3/flash_api.cpp:573.
@@ -330,6 +353,66 @@ typedef struct {
 
 int    fa_scheduler_metadata(const fa_sched_params* p);
 size_t fa_scheduler_metadata_ints(int32_t b);
+
+/* ------------------------------------------------------------------------
+ * Pages of a KV cache.  No counterpart in the reference, whose cache calls take a
+ * page table as it is given (flash_api.cpp:356).  `refs` holds one reference count
+ * a page; a page is free when it is 0.  Table rows are filled from the left, -1 =
+ * no page.  All of it runs on the stream; nothing is read on the host.
+ *   fa_pages_reserve  table entries below ceil((seqlens[r] + extra) / page_size)
+ *                     that are -1 get the lowest free pages, in the order of rows
+ *                     and entries; *missing = entries that stayed -1 for want of pages
+ *   fa_pages_free     entries from ceil((seqlens[r] + extra) / page_size) on (all,
+ *                     when seqlens is null) drop their page and become -1
+ *   fa_pages_fork     row i of new_table / new_seqlens (n rows) continues row
+ *                     rows[i] of the old table: full pages are shared, a partly
+ *                     filled last page goes to the last holder, the others get a copy
+ *                     of its rows in the lowest free pages (all of them when anyone
+ *                     outside these rows holds it, as with keep_parents); entries
+ *                     behind the length are -1.  keep_parents = 0: the old rows let
+ *                     go of all their pages.  A row number outside the old table
+ *                     makes an empty row; without a free page the row ends with its
+ *                     last full page and *missing counts it.
+ *   fa_pages_copy     page rows[i] -> page rows2[i] in every cache (pairs outside the
+ *                     pool are skipped; a page that is written may not be named twice)
+ *   fa_cache_compact  row seqlens[r] + kept[r][i] of the sequence becomes row
+ *                     seqlens[r] + i for i < counts[r], kept = rows (b, n) strictly
+ *                     increasing, counts = rows2 (null: n); ends at the first entry
+ *                     out of order or past the capacity; new_seqlens = seqlens + moved.
+ *                     table null: dense caches, num_pages entries of page_size rows.
+ * ---------------------------------------------------------------------- */
+typedef struct {                     /* one cache, or `caches` of them stride_cache apart; strides in BYTES */
+    void*   ptr;
+    int64_t stride_cache, stride_page, stride_row, stride_head;
+    int32_t caches, heads, segment_bytes;      /* a row: `heads` contiguous segments                */
+} fa_cache_view;
+
+typedef struct {
+    const fa_cache_view* caches;     /* HOST array                                          */
+    int32_t num_caches, num_pages, page_size;
+    int32_t* refs;                   /* (num_pages)                                         */
+    int32_t* table;                  /* (b, width), row stride table_stride                  */
+    int64_t  table_stride;
+    int32_t  b, width, extra, n, keep_parents;
+    const int32_t* seqlens;          /* (b)                                                 */
+    const int32_t* rows;             /* fork: parents (n); copy: src (n); compact: kept (b, n) */
+    const int32_t* rows2;            /* copy: dst (n); compact: counts (b) or null            */
+    int64_t  rows_stride;            /* of kept                                             */
+    const int32_t* cache_batch_idx;  /* compact, dense caches                                */
+    int32_t* new_table;              /* fork: (n, width) contiguous                          */
+    int32_t* new_seqlens;
+    int32_t* missing;                /* (1)                                                 */
+    void*    workspace;              /* reserve, fork: fa_pages_workspace_bytes(b or n, num_pages) */
+    size_t   workspace_bytes;
+    void*    stream;
+} fa_pages_params;
+
+int    fa_pages_reserve(const fa_pages_params* p);
+int    fa_pages_free(const fa_pages_params* p);
+int    fa_pages_fork(const fa_pages_params* p);
+int    fa_pages_copy(const fa_pages_params* p);
+int    fa_cache_compact(const fa_pages_params* p);
+size_t fa_pages_workspace_bytes(int32_t rows, int32_t num_pages);
 
 /* host-only helpers */
 const char* fa_last_error(void);
