@@ -46,6 +46,9 @@ void plan_forward(const fa_fwd_params& p, FwdPlan& plan);
 // kernels' host launchers (each returns an fa_status)
 int launch_fwd_generic(const fa_fwd_params& p, const FwdPlan& plan, float* o_part, float* lse_part);
 struct TreeMask;                                     // tree_mask.cuh
+bool fwd_sm100_tree_supported(const fa_fwd_params& p);
+long fwd_sm100_tree_ctas(const fa_fwd_params& p);     // CTAs of one key split
+int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, float* o_part, float* lse_part);
 int launch_fwd_generic_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, float* o_part, float* lse_part);
 int launch_fwd_decode(const fa_fwd_params& p, const FwdPlan& plan, float* o_part, float* lse_part);
 bool fwd_decode_supported(const fa_fwd_params& p);

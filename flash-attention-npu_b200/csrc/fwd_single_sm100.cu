@@ -92,12 +92,13 @@ __device__ __forceinline__ float2 tanh_small2(float2 y) {
 // tanh(y) for any y2e = 2 y log2(e): 1 - 2 / (1 + e^(2y)), absolute error about 1.8e-7
 __device__ __forceinline__ float tanh_any(float y2e) { return 1.f - __fdividef(2.f, 1.f + ex2_approx(y2e)); }
 
-template <typename T, int D>
+// TREE: the queries are drafted tokens behind a cache, rows of the tile are stacked rows (see Sm100FwdArgs)
+template <typename T, int D, bool TREE>
 __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_constant__ Sm100FwdArgs a) {
-    using L = FwdSingleSmem<D>;
+    using SM = FwdSingleSmem<D>;
     constexpr int NSUB = D / 64;
     constexpr int KSTEPS = D / 16;
-    constexpr int NST = L::kStages;
+    constexpr int NST = SM::kStages;
     constexpr bool kOwnP = D == 64;                          // P has columns of its own (see the head of the file)
     constexpr uint32_t TMEM_COLS = 256, COL_P = kOwnP ? 128 : 0, COL_O = kOwnP ? 192 : 128;
     constexpr uint32_t P_HALF = kOwnP ? 32 : 64;             // columns from the first to the second half of P
@@ -109,10 +110,10 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
     extern __shared__ unsigned char smem_raw[];
     const uint32_t sbase = (smem_addr(smem_raw) + 1023u) & ~1023u;
     unsigned char* sgen = smem_raw + (sbase - smem_addr(smem_raw));
-    const uint32_t sQ = sbase + L::oQ, sK = sbase + L::oK, sV = sbase + L::oV;
-    const uint32_t bars = sbase + L::oBar;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + L::oBar + 8 * N_COUNT);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + L::oBar + 8 * N_COUNT + 8);
+    const uint32_t sQ = sbase + SM::oQ, sK = sbase + SM::oK, sV = sbase + SM::oV;
+    const uint32_t bars = sbase + SM::oBar;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + SM::oBar + 8 * N_COUNT);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + SM::oBar + 8 * N_COUNT + 8);
     auto bar = [&](int i) { return bars + 8u * i; };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -122,25 +123,32 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
     const int b = pair / a.nheads_grid, hg = pair % a.nheads_grid;
     const int gq = a.gq;
     const int qpt = 128 / gq;                                // query positions of the tile
-    const int hk = gq > 1 ? hg : hg / (a.hq / a.hkv);
+    const int hk = TREE || gq > 1 ? hg : hg / (a.hq / a.hkv);
     const int h0 = gq > 1 ? hk * gq : hg;                    // head of tile row 0
     const int split = (int)blockIdx.y % a.nsplit;
     const int mblk = (int)gridDim.y / a.nsplit - 1 - (int)blockIdx.y / a.nsplit;
     int q_off = 0, k_off = 0, sq = a.sq, sk = a.sk;
     if (a.cu_q) { q_off = a.cu_q[b]; sq = a.cu_q[b + 1] - q_off; k_off = a.cu_k[b]; sk = a.cu_k[b + 1] - k_off; }
-    if (a.seqused_k) sk = (int)max(0LL, min((long long)a.seqused_k[b] + a.s_new, (long long)a.sk));
-    const int m0 = mblk * qpt;                               // first query position of the CTA
-    if (m0 >= sq) return;
+    int L = 0;                                               // TREE: cached rows in front of the draft
+    if constexpr (TREE) {
+        L = tree_prefix(a.seqused_k, b, a.sk);
+        sk = (int)min((long long)L + sq, (long long)a.sk);
+    } else if (a.seqused_k) sk = (int)max(0LL, min((long long)a.seqused_k[b] + a.s_new, (long long)a.sk));
+    const int r0 = TREE ? mblk * 128 : 0;                    // TREE: first stacked row of the CTA
+    const int m0 = TREE ? 0 : mblk * qpt;                    // first query position of the CTA
+    if (m0 >= sq || (TREE && r0 >= sq * gq)) return;
     if (g_fwd_single_error) return;
     const int wl = a.wl, wr = a.causal ? 0 : a.wr;
-    const int rows = min(128, (sq - m0) * gq);               // tile rows in use
+    const int rows = min(128, (sq - m0) * gq - r0);          // tile rows in use
 
     int lo_first, hi_first, lo_last, hi_last;
     window_bounds(m0, sq, sk, wl, wr, lo_first, hi_first);
     window_bounds(m0 + (rows - 1) / gq, sq, sk, wl, wr, lo_last, hi_last);
     int t_lo = lo_first / 128, t_hi = hi_last < 0 ? 0 : hi_last / 128 + 1;
     if (sk <= 0 || lo_first >= sk) { t_lo = 0; t_hi = 0; }
-    if (a.nsplit > 1) {                                      // this split's share of the key tiles
+    if constexpr (TREE) {
+        tree_split_tiles(tree_first_any(a.tree, L), sk, a.nsplit, split, a.min_split_keys, t_lo, t_hi);
+    } else if (a.nsplit > 1) {                               // this split's share of the key tiles
         t_lo = max(t_lo, split * (a.keys_per_split / 128));
         t_hi = min(t_hi, (split + 1) * (a.keys_per_split / 128));
     }
@@ -148,12 +156,15 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
 
     // output row, LSE slot and row in the partial buffers of tile row t
     auto out_row = [&](int t) -> T* {
+        t += r0;
         return reinterpret_cast<T*>(a.o) + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(q_off + m0 + t / gq) * a.o_ss + (int64_t)(h0 + t % gq) * a.o_sh;
     };
     auto lse_slot = [&](int t) -> float* {
+        t += r0;
         return a.lse + (a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)(h0 + t % gq) * a.lse_sh + (int64_t)(q_off + m0 + t / gq) * a.lse_ss;
     };
     auto part_row = [&](int t) -> int64_t {
+        t += r0;
         return (int64_t)split * a.rows_all + ((int64_t)b * a.sq + m0 + t / gq) * a.hq + h0 + t % gq;
     };
 
@@ -188,21 +199,37 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
     const uint32_t tmem = *tmem_slot;
     int* err = &g_fwd_single_error;
 
-    if (warp == 8) {
+    if (TREE && warp == 8) {
+        if (lane == 0) {
+            mbar_expect_tx(bar(N_Q), SM::kTile);
+#pragma unroll
+            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * SM::kSub, &a.tq, bar(N_Q), s * 64, hk, r0, b);
+        }
+        bool ok = true;                                      // the whole warp, one lane a box: lanes leave together
+        for (int j = 0; j < ntiles && ok; ++j) {
+            const int st = j % NST, use = j / NST;
+            if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(N_KE0 + st), (use - 1) & 1, abort_flag, err, 81));
+            if (!ok) break;
+            tree_load_tile<NSUB>(a, &a.tk, sK + st * SM::kTile, bar(N_KF0 + st), (t_lo + j) * 128, hk, b, lane);
+            if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(N_VE0 + st), (use - 1) & 1, abort_flag, err, 82));
+            if (!ok) break;
+            tree_load_tile<NSUB>(a, &a.tv, sV + st * SM::kTile, bar(N_VF0 + st), (t_lo + j) * 128, hk, b, lane);
+        }
+    } else if (warp == 8) {
         if (lane == 0) {
             tma_prefetch_desc(&a.tq); tma_prefetch_desc(&a.tk); tma_prefetch_desc(&a.tv);
-            mbar_expect_tx(bar(N_Q), L::kTile);
+            mbar_expect_tx(bar(N_Q), SM::kTile);
 #pragma unroll
-            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * L::kSub, &a.tq, bar(N_Q), s * 64, h0, (a.cu_q ? q_off : 0) + m0, a.cu_q ? 0 : b);
+            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * SM::kSub, &a.tq, bar(N_Q), s * 64, h0, (a.cu_q ? q_off : 0) + m0, a.cu_q ? 0 : b);
             // where key tile j lives: as in the two-tile kernel
             const int32_t* btab = a.block_table ? a.block_table + (int64_t)b * a.bt_stride : nullptr;
             const int kbatch = a.cu_q ? 0 : (a.cache_batch_idx ? a.cache_batch_idx[b] : b);
             auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t full, int krow, int kouter, int krow2, int kouter2) {
-                mbar_expect_tx(full, L::kTile);
+                mbar_expect_tx(full, SM::kTile);
 #pragma unroll
                 for (int s = 0; s < NSUB; ++s) {
-                    tma_load_4d(dst + s * L::kSub, map, full, s * 64, hk, krow, kouter);
-                    if (a.kv_box == 64) tma_load_4d(dst + s * L::kSub + 64 * 128, map, full, s * 64, hk, krow2, kouter2);
+                    tma_load_4d(dst + s * SM::kSub, map, full, s * 64, hk, krow, kouter);
+                    if (a.kv_box == 64) tma_load_4d(dst + s * SM::kSub + 64 * 128, map, full, s * 64, hk, krow2, kouter2);
                 }
             };
             bool ok = true;
@@ -221,16 +248,16 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
                 }
                 if (use > 0) ok = mbar_wait(bar(N_KE0 + st), (use - 1) & 1, abort_flag, err, 81);
                 if (!ok) break;
-                load(sK + st * L::kTile, &a.tk, bar(N_KF0 + st), krow, kouter, krow2, kouter2);
+                load(sK + st * SM::kTile, &a.tk, bar(N_KF0 + st), krow, kouter, krow2, kouter2);
                 if (use > 0) ok = mbar_wait(bar(N_VE0 + st), (use - 1) & 1, abort_flag, err, 82);
                 if (!ok) break;
-                load(sV + st * L::kTile, &a.tv, bar(N_VF0 + st), krow, kouter, krow2, kouter2);
+                load(sV + st * SM::kTile, &a.tv, bar(N_VF0 + st), krow, kouter, krow2, kouter2);
             }
         }
     } else if (warp == 9) {
-        const uint64_t dQ = umma_desc(sQ, 16, 1024), dK = umma_desc(sK, 16, 1024), dV = umma_desc(sV, L::kSub, 1024);
+        const uint64_t dQ = umma_desc(sQ, 16, 1024), dK = umma_desc(sK, 16, 1024), dV = umma_desc(sV, SM::kSub, 1024);
         auto issue_qk = [&](int j) {
-            umma_ss_scores<KSTEPS, L::kSub>(tmem, dQ, umma_desc_at(dK, (j % NST) * L::kTile), IDESC_QK);
+            umma_ss_scores<KSTEPS, SM::kSub>(tmem, dQ, umma_desc_at(dK, (j % NST) * SM::kTile), IDESC_QK);
             umma_commit_w(bar(N_S));
             umma_commit_w(bar(N_KE0 + j % NST));
         };
@@ -251,7 +278,8 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
             ok = mbar_wait(bar(N_VF0 + st), (j / NST) & 1, abort_flag, err, 86);
             if (!kOwnP && ok && more) ok = mbar_wait(bar(N_KF0 + (j + 1) % NST), ((j + 1) / NST) & 1, abort_flag, err, 87);
             if (!ok) break;
-            if (a.seqused_k && (t_lo + j) * 128 + 128 > sk) {
+            if constexpr (TREE) tree_clear_rows<NSUB>(a, sgen + SM::oV + st * SM::kTile, (t_lo + j) * 128, L, b, lane);
+            else if (a.seqused_k && (t_lo + j) * 128 + 128 > sk) {
                 // cache rows past the sequence may hold NaN patterns and 0 x NaN is NaN: the V rows that the copy fetched
                 // are cleared (rows past the capacity of a dense cache were zero-filled by the copy)
                 const int first = max(0, sk - (t_lo + j) * 128);
@@ -259,7 +287,7 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
 #pragma unroll
                 for (int sub = 0; sub < NSUB; ++sub)
                     for (int idx = first * 8 + lane; idx < last * 8; idx += 32)
-                        *reinterpret_cast<uint4*>(sgen + L::oV + st * L::kTile + sub * L::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(sgen + SM::oV + st * SM::kTile + sub * SM::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async_smem();
                 __syncwarp();
             }
@@ -267,7 +295,7 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
             if (!ok) break;
             tc_fence_after();
             // 16 keys = 8 columns of P and 2048 bytes of V a step; keys 0-31 and 64-95, then 32-63 and 96-127
-            const uint64_t bv = umma_desc_at(dV, st * L::kTile);
+            const uint64_t bv = umma_desc_at(dV, st * SM::kTile);
             umma_ts_quad<0, 8, P_HALF, P_HALF + 8, 0, 128, 512, 640>(tmem + COL_O, tmem + COL_P, bv, IDESC_PV, j > 0);
             ok = mbar_wait(bar(N_P1), j & 1, abort_flag, err, 91);
             if (!ok) break;
@@ -291,15 +319,27 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
         const uint32_t t_s = tmem + lane_base + half * 64;
         const uint32_t t_p = tmem + lane_base + COL_P + half * P_HALF;
         const uint32_t t_o = tmem + lane_base + COL_O + half * (D / 2);     // the half of O this thread rescales and stores
-        float* s_max = reinterpret_cast<float*>(sgen + L::oMax);
-        float* s_sum = reinterpret_cast<float*>(sgen + L::oSum);
-        const int qi = m0 + r / gq;
+        float* s_max = reinterpret_cast<float*>(sgen + SM::oMax);
+        float* s_sum = reinterpret_cast<float*>(sgen + SM::oSum);
+        const int qi = m0 + (r0 + r) / gq;
         int klo = 1, khi = 0;
-        if (r < rows) window_bounds(qi, sq, sk, wl, wr, klo, khi);
+        const uint32_t* tree_row = nullptr;
+        bool there = true;                                   // TREE: the row's token exists
+        if constexpr (TREE) {
+            klo = 0x7fffffff;
+            if (r < rows) {
+                klo = tree_first_key(a.tree, b, qi, L);
+                tree_row = a.tree.bits + (int64_t)(b * a.tree.tokens + qi) * a.tree.words;
+            }
+            there = klo != 0x7fffffff;
+        } else if (r < rows) window_bounds(qi, sq, sk, wl, wr, klo, khi);
         // key range that every / any row of this warp sees (rows past the end see nothing and only lose the fast path)
         const int wfirst = quarter * 32, wlast = min(wfirst + 31, rows - 1);
         int all_lo = 1, all_hi = 0, any_lo = 1, any_hi = 0;
-        if (wfirst < rows) {
+        if constexpr (TREE) {
+            all_lo = tree_first_all(a.tree, L); all_hi = L - 1;
+            any_lo = tree_first_any(a.tree, L); any_hi = sk - 1;
+        } else if (wfirst < rows) {
             int tl, th;
             window_bounds(m0 + wfirst / gq, sq, sk, wl, wr, any_lo, all_hi);
             window_bounds(m0 + wlast / gq, sq, sk, wl, wr, tl, th);
@@ -332,7 +372,16 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
             }
             // every score of the warp is in the range of the tanh polynomial
             const bool small = __all_sync(0xffffffffu, fmaxf(a0, a1) * a.cap_in <= kTanhSmall);
-            auto seen = [&](int c, int i) { const int col = n0 + c * 32 + i; return col >= klo && col <= khi; };
+            uint32_t vis[2] = {~0u, ~0u};
+            if (TREE && !full) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) vis[c] = there ? tree_visible32(a.tree, tree_row, n0 + c * 32, klo, L) : 0u;
+            }
+            auto seen = [&](int c, int i) {
+                if constexpr (TREE) return (vis[c] >> i & 1) != 0;
+                const int col = n0 + c * 32 + i;
+                return col >= klo && col <= khi;
+            };
             if (!full) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -355,7 +404,8 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
             float m_loc = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
             // the cap is monotone; log2 domain.  It makes a finite score of an infinite one, so that -inf only stands for a row
             // that sees none of these keys.
-            m_loc = klo <= khi && klo <= n0 + 63 && khi >= n0 ? cap_out * tanh_any(m_loc * cap_in2) : -INFINITY;
+            const bool any_seen = TREE ? (vis[0] | vis[1]) != 0 : klo <= khi && klo <= n0 + 63 && khi >= n0;
+            m_loc = any_seen ? cap_out * tanh_any(m_loc * cap_in2) : -INFINITY;
             // one of the 64 threads moves its base (or gave up waiting): both warps take the slow way
             if (pair_any(bid, !ok || m_loc > m_used + kRescaleThreshold)) {
                 s_max[half * 128 + r] = m_loc;
@@ -430,7 +480,7 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
         // the two halves of the row sum (after a break both warps come here with `ok` false)
         s_sum[half * 128 + r] = l_run;
         ok = !pair_any(bid, !ok);
-        const float l_tot = s_sum[r] + s_sum[128 + r];
+        const float l_tot = TREE && !there ? 0.f : s_sum[r] + s_sum[128 + r];
         if (ok) ok = mbar_wait(bar(N_O), 0, abort_flag, err, 90);
         if (ok) {
             tc_fence_after();
@@ -443,6 +493,12 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
                 uint32_t oreg[32];
                 tmem_ld32(t_o + c * 32, oreg);
                 tmem_wait_ld();
+                if constexpr (TREE) {
+                    if (!there) {                            // no token: whatever its q holds, zeros
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) oreg[i] = 0u;
+                    }
+                }
                 if (r < rows && prow) {
 #pragma unroll
                     for (int v = 0; v < 8; ++v)
@@ -473,16 +529,16 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TREE>
 int launch_t(const fa_fwd_params& p, Sm100FwdArgs& a) {
     cudaStream_t st = reinterpret_cast<cudaStream_t>(p.stream);
-    auto kern = fwd_single_sm100_kernel<T, D>;
+    auto kern = fwd_single_sm100_kernel<T, D, TREE>;
     const int smem = FwdSingleSmem<D>::kBytes + 1024;
     if (int e = cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return e;
     if (int e = cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared), "cudaFuncSetAttribute")) return e;
     const int qpc = 128 / a.gq;                              // query positions of a CTA
-    const unsigned nbx = (unsigned)(((p.sq + qpc - 1) / qpc) * a.nsplit);
-    a.nheads_grid = a.gq > 1 ? p.hkv : p.hq;
+    const unsigned nbx = (unsigned)((TREE ? (p.sq * a.gq + 127) / 128 : (p.sq + qpc - 1) / qpc) * a.nsplit);
+    a.nheads_grid = TREE || a.gq > 1 ? p.hkv : p.hq;
     a.chunk = grid_chunk((int64_t)p.b * a.nheads_grid, (int64_t)p.sk * p.d * 4);
     dim3 grid(a.chunk, nbx, (unsigned)(((int64_t)p.b * a.nheads_grid + a.chunk - 1) / a.chunk));
     kern<<<grid, 320, smem, st>>>(a);
@@ -491,9 +547,13 @@ int launch_t(const fa_fwd_params& p, Sm100FwdArgs& a) {
 }
 }  // namespace
 
-int launch_fwd_single_sm100(const fa_fwd_params& p, Sm100FwdArgs& a) {
-    if (p.dtype == FA_F16) return p.d <= 64 ? launch_t<__half, 64>(p, a) : launch_t<__half, 128>(p, a);
-    return p.d <= 64 ? launch_t<__nv_bfloat16, 64>(p, a) : launch_t<__nv_bfloat16, 128>(p, a);
+template <bool TREE>
+static int launch_dims(const fa_fwd_params& p, Sm100FwdArgs& a) {
+    if (p.dtype == FA_F16) return p.d <= 64 ? launch_t<__half, 64, TREE>(p, a) : launch_t<__half, 128, TREE>(p, a);
+    return p.d <= 64 ? launch_t<__nv_bfloat16, 64, TREE>(p, a) : launch_t<__nv_bfloat16, 128, TREE>(p, a);
+}
+int launch_fwd_single_sm100(const fa_fwd_params& p, Sm100FwdArgs& a, bool tree) {
+    return tree ? launch_dims<true>(p, a) : launch_dims<false>(p, a);
 }
 
 }  // namespace fa

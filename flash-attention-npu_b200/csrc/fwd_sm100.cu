@@ -31,6 +31,8 @@ __device__ int g_fwd_sm100_error = 0;
 // groups and both accumulators work on the SAME rows, group A on the even key tiles and group B on the odd ones, and the two
 // partial results are merged in the epilogue.  With one tile in flight the K and V stream stood still while that tile went
 // through QK^T, softmax and PV.
+//
+// TREE: the queries are drafted tokens behind a cache (see Sm100FwdArgs), of which 128 or 256 stacked rows make a CTA.
 // =================================================================================================
 template <int D, bool DUAL>
 struct FwdSm100Smem2 {
@@ -54,10 +56,10 @@ struct FwdSm100Smem2 {
 template <int D> constexpr int kFwdPoly = D == 128 ? 1 : 2;
 enum { C_Q = 0, C_KF0, C_KF1, C_KF2, C_KE0, C_KE1, C_KE2, C_VF0, C_VF1, C_VF2, C_VE0, C_VE1, C_VE2, C_SA, C_SB, C_PA, C_PB, C_PA2, C_PB2, C_OA, C_OB, C_DRAIN, C_COUNT };
 
-template <typename T, int D, bool BIAS, bool DUAL>
+template <typename T, int D, bool BIAS, bool DUAL, bool TREE>
 __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constant__ Sm100FwdArgs a) {
-    using L = FwdSm100Smem2<D, DUAL>;
-    constexpr int NST = L::kStages;
+    using SM = FwdSm100Smem2<D, DUAL>;
+    constexpr int NST = SM::kStages;
     constexpr int NSUB = D / 64;
     constexpr int KSTEPS = D / 16;
     constexpr uint32_t TMEM_COLS = 512;
@@ -69,10 +71,10 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     extern __shared__ unsigned char smem_raw[];
     const uint32_t sbase = (smem_addr(smem_raw) + 1023u) & ~1023u;
     unsigned char* sgen = smem_raw + (sbase - smem_addr(smem_raw));
-    const uint32_t sQ = sbase + L::oQ, sK = sbase + L::oK, sV = sbase + L::oV;
-    const uint32_t bars = sbase + L::oBar;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + L::oBar + 8 * C_COUNT);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + L::oBar + 8 * C_COUNT + 8);
+    const uint32_t sQ = sbase + SM::oQ, sK = sbase + SM::oK, sV = sbase + SM::oV;
+    const uint32_t bars = sbase + SM::oBar;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + SM::oBar + 8 * C_COUNT);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + SM::oBar + 8 * C_COUNT + 8);
     auto bar = [&](int i) { return bars + 8u * i; };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -101,14 +103,19 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     const int mblk = nbx / a.nsplit - 1 - bi.x / a.nsplit;
     int q_off = 0, k_off = 0, sq = a.sq, sk = a.sk;
     if (a.cu_q) { q_off = a.cu_q[b]; sq = a.cu_q[b + 1] - q_off; k_off = a.cu_k[b]; sk = a.cu_k[b + 1] - k_off; }
-    if (a.seqused_k) {                                       // cache call: the length lives on the device
+    int L = 0;                                               // TREE: cached rows in front of the draft
+    if constexpr (TREE) {
+        L = tree_prefix(a.seqused_k, b, a.sk);
+        sk = (int)min((long long)L + sq, (long long)a.sk);
+    } else if (a.seqused_k) {                                // cache call: the length lives on the device
         sk = (int)max(0LL, min((long long)a.seqused_k[b] + a.s_new, (long long)a.sk));   // an oversized entry is truncated to the capacity
     }
-    const int m0 = mblk * (DUAL ? 1 : 2) * qpt;              // first query position of the CTA
-    if (m0 >= sq) return;
+    const int r0 = TREE ? mblk * (DUAL ? 128 : 256) : 0;     // TREE: first stacked row of the CTA
+    const int m0 = TREE ? 0 : mblk * (DUAL ? 1 : 2) * qpt;   // first query position of the CTA
+    if (m0 >= sq || (TREE && r0 >= sq * gq)) return;
     if (failed) return;
     const int wl = a.wl, wr = a.causal ? 0 : a.wr;
-    const int rows_cta = min(DUAL ? 128 : 256, (sq - m0) * gq);          // tile rows in use
+    const int rows_cta = min(DUAL ? 128 : 256, (sq - m0) * gq - r0);     // tile rows in use
     const bool has_b = !DUAL && rows_cta > 128;
 
     int lo_first, hi_first, lo_last, hi_last;
@@ -116,7 +123,9 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     window_bounds(m0 + (rows_cta - 1) / gq, sq, sk, wl, wr, lo_last, hi_last);
     int t_lo = lo_first / 128, t_hi = hi_last < 0 ? 0 : hi_last / 128 + 1;
     if (sk <= 0 || lo_first >= sk) { t_lo = 0; t_hi = 0; }
-    if (a.nsplit > 1) {                                      // this split's share of the key tiles
+    if constexpr (TREE) {
+        tree_split_tiles(tree_first_any(a.tree, L), sk, a.nsplit, split, a.min_split_keys, t_lo, t_hi);
+    } else if (a.nsplit > 1) {                               // this split's share of the key tiles
         t_lo = max(t_lo, split * (a.keys_per_split / 128));
         t_hi = min(t_hi, (split + 1) * (a.keys_per_split / 128));
     }
@@ -124,7 +133,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     // The first 128 rows of the block may end before the last key tile of the block (under a causal mask they end one
     // tile earlier): they skip the tiles in which every one of their entries is masked.
     int nt0 = ntiles;
-    if (has_b) {
+    if (!TREE && has_b) {
         int lo_a, hi_a;
         window_bounds(m0 + qpt - 1, sq, sk, wl, wr, lo_a, hi_a);
         const int n = min(ntiles, (hi_a < 0 ? 0 : hi_a / 128 + 1) - t_lo);
@@ -133,13 +142,16 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
 
     // output row and LSE slot of tile row t (0..255) of this CTA
     auto out_row = [&](int t) -> T* {
+        t += r0;
         return reinterpret_cast<T*>(a.o) + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(q_off + m0 + t / gq) * a.o_ss + (int64_t)(h0 + t % gq) * a.o_sh;
     };
     auto lse_slot = [&](int t) -> float* {
+        t += r0;
         return a.lse + (a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)(h0 + t % gq) * a.lse_sh + (int64_t)(q_off + m0 + t / gq) * a.lse_ss;
     };
     // split-KV: row of tile row t in the partial buffers
     auto part_row = [&](int t) -> int64_t {
+        t += r0;
         return (int64_t)split * a.rows_all + ((int64_t)b * a.sq + m0 + t / gq) * a.hq + h0 + t % gq;
     };
 
@@ -159,8 +171,9 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
         return;
     }
 
-    const int qrow0 = (a.cu_q ? q_off : 0) + m0;
+    const int qrow0 = TREE ? r0 : (a.cu_q ? q_off : 0) + m0;
     const int qb = a.cu_q ? 0 : b;
+    const int qh = TREE ? hk : h0, qrow1 = qrow0 + (TREE ? 128 : qpt);
     // where key tile j lives: (row, outermost coordinate) of the K / V maps.  Dense and packed operands: row
     // in the batch entry; cache: row in the cache entry of this batch; paged cache: row inside the page
     // that the page table names (a tile never straddles pages when the page size is a multiple of 128; pages of
@@ -184,11 +197,11 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
         }
     };
     auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int krow, int kouter, int krow2, int kouter2) {
-        mbar_expect_tx(full, L::kKV);
+        mbar_expect_tx(full, SM::kKV);
 #pragma unroll
         for (int s = 0; s < NSUB; ++s) {
-            tma_load_4d(dst + s * L::kSub, map, full, s * 64, hk, krow, kouter);
-            if (a.kv_box == 64) tma_load_4d(dst + s * L::kSub + 64 * 128, map, full, s * 64, hk, krow2, kouter2);
+            tma_load_4d(dst + s * SM::kSub, map, full, s * 64, hk, krow, kouter);
+            if (a.kv_box == 64) tma_load_4d(dst + s * SM::kSub + 64 * 128, map, full, s * 64, hk, krow2, kouter2);
         }
     };
     if (warp == 8) {
@@ -199,19 +212,25 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
             for (int i = 0; i < C_COUNT; ++i) mbar_init(bar(i), (i >= C_PA && i <= C_PB2) ? 128u : 1u);
             *abort_flag = 0;
             mbar_fence_init();
-            mbar_expect_tx(bar(C_Q), has_b ? 2 * L::kQ : L::kQ);
+            mbar_expect_tx(bar(C_Q), has_b ? 2 * SM::kQ : SM::kQ);
 #pragma unroll
-            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * L::kSub, &a.tq, bar(C_Q), s * 64, h0, qrow0, qb);
+            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * SM::kSub, &a.tq, bar(C_Q), s * 64, qh, qrow0, qb);
             int krow, kouter, krow2, kouter2;
-            place(0, krow, kouter, krow2, kouter2);
-            load(&a.tk, sK, bar(C_KF0), krow, kouter, krow2, kouter2);
+            if constexpr (!TREE) {
+                place(0, krow, kouter, krow2, kouter2);
+                load(&a.tk, sK, bar(C_KF0), krow, kouter, krow2, kouter2);
+            }
             if (has_b) {
 #pragma unroll
-                for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + L::kQ + s * L::kSub, &a.tq, bar(C_Q), s * 64, h0, qrow0 + qpt, qb);
+                for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + SM::kQ + s * SM::kSub, &a.tq, bar(C_Q), s * 64, qh, qrow1, qb);
             }
-            load(&a.tv, sV, bar(C_VF0), krow, kouter, krow2, kouter2);
+            if constexpr (!TREE) load(&a.tv, sV, bar(C_VF0), krow, kouter, krow2, kouter2);
         }
         __syncwarp();
+        if constexpr (TREE) {
+            tree_load_tile<NSUB>(a, &a.tk, sK, bar(C_KF0), t_lo * 128, hk, b, lane);
+            tree_load_tile<NSUB>(a, &a.tv, sV, bar(C_VF0), t_lo * 128, hk, b, lane);
+        }
         tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
         tmem_relinquish();
     }
@@ -228,7 +247,18 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     static_assert(128 * 56 + 256 * 224 <= 384 * 168, "register split exceeds the CTA's allocation");
     if (warp >= 8) {
     reg_dealloc<56>();
-    if (warp == 8) {
+    if (TREE && warp == 8) {
+        bool ok = true;                                      // the whole warp, one lane a box: lanes leave together
+        for (int j = 1; j < ntiles && ok; ++j) {
+            const int st = j % NST, use = j / NST;
+            if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(C_KE0 + st), (use - 1) & 1, abort_flag, err, 1));
+            if (!ok) break;
+            tree_load_tile<NSUB>(a, &a.tk, sK + st * SM::kKV, bar(C_KF0 + st), (t_lo + j) * 128, hk, b, lane);
+            if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(C_VE0 + st), (use - 1) & 1, abort_flag, err, 2));
+            if (!ok) break;
+            tree_load_tile<NSUB>(a, &a.tv, sV + st * SM::kKV, bar(C_VF0 + st), (t_lo + j) * 128, hk, b, lane);
+        }
+    } else if (warp == 8) {
         if (lane == 0) {
             bool ok = true;
             for (int j = 1; j < ntiles && ok; ++j) {
@@ -237,24 +267,24 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                 place(j, krow, kouter, krow2, kouter2);
                 if (use > 0) ok = mbar_wait(bar(C_KE0 + st), (use - 1) & 1, abort_flag, err, 1);
                 if (!ok) break;
-                load(&a.tk, sK + st * L::kKV, bar(C_KF0 + st), krow, kouter, krow2, kouter2);
+                load(&a.tk, sK + st * SM::kKV, bar(C_KF0 + st), krow, kouter, krow2, kouter2);
                 if (use > 0) ok = mbar_wait(bar(C_VE0 + st), (use - 1) & 1, abort_flag, err, 2);
                 if (!ok) break;
-                load(&a.tv, sV + st * L::kKV, bar(C_VF0 + st), krow, kouter, krow2, kouter2);
+                load(&a.tv, sV + st * SM::kKV, bar(C_VF0 + st), krow, kouter, krow2, kouter2);
             }
         }
     } else if (warp == 9) {
         {   // whole warp, one elected lane issues (see umma_ss_w)
             // descriptors of the tile origins, built once; the grouped issue adds compile-time offsets
-            const uint64_t dQ0 = umma_desc(sQ, 16, 1024), dK0 = umma_desc(sK, 16, 1024), dV0 = umma_desc(sV, L::kSub, 1024);
+            const uint64_t dQ0 = umma_desc(sQ, 16, 1024), dK0 = umma_desc(sK, 16, 1024), dV0 = umma_desc(sV, SM::kSub, 1024);
             auto issue_qk = [&](int x, int st) {
-                umma_ss_scores<KSTEPS, L::kSub>(tmem + x * 128, umma_desc_at(dQ0, x * L::kQ), umma_desc_at(dK0, st * L::kKV), IDESC_QK);
+                umma_ss_scores<KSTEPS, SM::kSub>(tmem + x * 128, umma_desc_at(dQ0, x * SM::kQ), umma_desc_at(dK0, st * SM::kKV), IDESC_QK);
                 umma_commit_w(bar(C_SA + x));
             };
             // P·V of tile x in two halves of 64 keys (16 keys = 8 columns of P, 2048 bytes of V a step): the second
             // half waits for its own barrier
             auto issue_pv = [&](int x, int st, int j) -> bool {
-                const uint64_t bv = umma_desc_at(dV0, st * L::kKV);
+                const uint64_t bv = umma_desc_at(dV0, st * SM::kKV);
                 const uint32_t d_o = tmem + 256 + x * 128, a_p = tmem + x * 128;
                 umma_ts_group4<0, 8, 0, 128>(d_o, a_p, bv, IDESC_PV, j > 0);
                 if (!mbar_wait(bar(C_PA2 + x), j & 1, abort_flag, err, 11)) return false;
@@ -266,13 +296,17 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
             if constexpr (DUAL) {
                 // stale V rows, as in the other form below
                 auto clear_stale = [&](int j, int st) {
+                    if constexpr (TREE) {
+                        tree_clear_rows<NSUB>(a, sgen + SM::oV + st * SM::kKV, (t_lo + j) * 128, L, b, lane);
+                        return;
+                    }
                     if (!a.seqused_k || (t_lo + j) * 128 + 128 <= sk) return;
                     const int first = max(0, sk - (t_lo + j) * 128);
                     const int last = a.block_table ? 128 : min(128, a.sk - (t_lo + j) * 128);
 #pragma unroll
                     for (int sub = 0; sub < NSUB; ++sub)
                         for (int idx = first * 8 + lane; idx < last * 8; idx += 32)     // 16-byte chunks of rows first .. last - 1
-                            *reinterpret_cast<uint4*>(sgen + L::oV + st * L::kKV + sub * L::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(sgen + SM::oV + st * SM::kKV + sub * SM::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
                     fence_proxy_async_smem();
                     __syncwarp();
                 };
@@ -280,7 +314,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                 auto scores = [&](int j) -> bool {
                     if (!mbar_wait(bar(C_KF0 + j % NST), (j / NST) & 1, abort_flag, err, 7)) return false;
                     tc_fence_after();
-                    umma_ss_scores<KSTEPS, L::kSub>(tmem + (j & 1) * 128, dQ0, umma_desc_at(dK0, (j % NST) * L::kKV), IDESC_QK);
+                    umma_ss_scores<KSTEPS, SM::kSub>(tmem + (j & 1) * 128, dQ0, umma_desc_at(dK0, (j % NST) * SM::kKV), IDESC_QK);
                     umma_commit_w(bar(C_SA + (j & 1)));
                     umma_commit_w(bar(C_KE0 + j % NST));
                     return true;
@@ -320,7 +354,8 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                 ok = mbar_wait(bar(C_VF0 + st), use & 1, abort_flag, err, 6);
                 if (ok && more) ok = mbar_wait(bar(C_KF0 + st1), use1 & 1, abort_flag, err, 7);
                 if (!ok) break;
-                if (a.seqused_k && (t_lo + j) * 128 + 128 > sk) {
+                if constexpr (TREE) tree_clear_rows<NSUB>(a, sgen + SM::oV + st * SM::kKV, (t_lo + j) * 128, L, b, lane);
+                else if (a.seqused_k && (t_lo + j) * 128 + 128 > sk) {
                     // Rows of a cache past the sequence hold whatever was there before (possibly NaN patterns): their
                     // probabilities are exact zeros, but 0 x NaN is NaN, so the V rows are cleared before the MMA.
                     // A row is 128 bytes in every 64-column sub-tile whatever the swizzle.
@@ -331,7 +366,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
 #pragma unroll
                     for (int sub = 0; sub < NSUB; ++sub)
                         for (int idx = first * 8 + lane; idx < last * 8; idx += 32)     // 16-byte chunks of rows first .. last - 1
-                            *reinterpret_cast<uint4*>(sgen + L::oV + st * L::kKV + sub * L::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(sgen + SM::oV + st * SM::kKV + sub * SM::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
@@ -381,12 +416,25 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
         const uint32_t t_s = tmem + lane_base + x * 128;
         const uint32_t t_o = tmem + lane_base + 256 + x * 128;
         const int rows = min(128, rows_cta - x0);
-        const int qi = m0 + (x0 + r) / gq;                  // query position of this thread's row
+        const int qi = m0 + (r0 + x0 + r) / gq;             // query position of this thread's row
         int klo = 1, khi = 0;
-        if (r < rows) window_bounds(qi, sq, sk, wl, wr, klo, khi);
         int lo_l, hi_f, tmp;
-        window_bounds(m0 + x0 / gq, sq, sk, wl, wr, tmp, hi_f);
-        window_bounds(m0 + (x0 + rows - 1) / gq, sq, sk, wl, wr, lo_l, tmp);
+        const uint32_t* tree_row = nullptr;
+        bool there = true;                                   // TREE: the row's token exists
+        if constexpr (TREE) {
+            klo = 0x7fffffff;
+            if (r < rows) {
+                klo = tree_first_key(a.tree, b, qi, L);
+                tree_row = a.tree.bits + (int64_t)(b * a.tree.tokens + qi) * a.tree.words;
+            }
+            there = klo != 0x7fffffff;
+            lo_l = tree_first_all(a.tree, L);                // tiles inside [lo_l, hi_f] are seen by every token
+            hi_f = L - 1;
+        } else {
+            if (r < rows) window_bounds(qi, sq, sk, wl, wr, klo, khi);
+            window_bounds(m0 + x0 / gq, sq, sk, wl, wr, tmp, hi_f);
+            window_bounds(m0 + (x0 + rows - 1) / gq, sq, sk, wl, wr, lo_l, tmp);
+        }
         float m_used = -INFINITY, l_run = 0.f;
         // BIAS instantiation: the scores are turned into their final log2-domain values in registers (softcap, then
         // alibi, as the general kernel and the golden do), and the softmax below runs with a unit scale
@@ -434,10 +482,12 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                 if (!full) {
 #pragma unroll
                     for (int c = 2 * hh; c < 2 * hh + 2; ++c) {
+                        uint32_t vis = 0;
+                        if constexpr (TREE) vis = there ? tree_visible32(a.tree, tree_row, n0 + c * 32, klo, L) : 0u;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const int col = n0 + c * 32 + i;
-                            if (col < klo || col > khi) sreg[c][i] = 0xff800000u;     // -inf
+                            if (TREE ? !(vis >> i & 1) : col < klo || col > khi) sreg[c][i] = 0xff800000u;     // -inf
                         }
                     }
                 }
@@ -510,7 +560,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
             // All MMAs are done, so every copy has landed and been read: the exponent bases and row sums of both groups go
             // through the K buffers.
             if (ok && ntiles > 1) ok = mbar_wait(bar(C_OB), 0, abort_flag, err, 12);
-            float* merge = reinterpret_cast<float*>(sgen + L::oK);
+            float* merge = reinterpret_cast<float*>(sgen + SM::oK);
             merge[x * 256 + r] = m_used;
             merge[x * 256 + 128 + r] = l_run;
             asm volatile("barrier.cta.sync 1, 256;" ::: "memory");               // both groups, whatever became of their waits
@@ -520,6 +570,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
             f_b = m_b == -INFINITY ? 0.f : ex2_approx(m_b - m_used);
             l_run = merge[128 + r] * f_a + merge[384 + r] * f_b;
         }
+        if (TREE && !there) l_run = 0.f;                         // no token: whatever its q holds, zeros and no LSE
         if (ok) {
             tc_fence_after();
             const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
@@ -541,6 +592,12 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                         tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; ++i) oreg[i] = __float_as_uint(fmaf(__uint_as_float(ob[i]), f_b, __uint_as_float(oreg[i])));
+                    }
+                }
+                if constexpr (TREE) {
+                    if (!there) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) oreg[i] = 0u;
                     }
                 }
                 if (r < rows && prow) {
@@ -593,9 +650,9 @@ struct FwdSm100SmemWide {
 };
 enum { W_Q = 0, W_KF, W_KE, W_VF, W_VE, W_S0, W_S1, W_P0, W_P1, W_P0B, W_P1B, W_O, W_COUNT };
 
-template <typename T, int D, bool BIAS>
+template <typename T, int D, bool BIAS, bool TREE>
 __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_constant__ Sm100FwdArgs a) {
-    using L = FwdSm100SmemWide<D>;
+    using SM = FwdSm100SmemWide<D>;
     constexpr int NSUB = D / 64;
     constexpr uint32_t TMEM_COLS = 512, COL_O = 256;
     constexpr int FMT = Elem<T>::kDtype == FA_BF16 ? 1 : 0;
@@ -606,45 +663,65 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
     extern __shared__ unsigned char smem_raw[];
     const uint32_t sbase = (smem_addr(smem_raw) + 1023u) & ~1023u;
     unsigned char* sgen = smem_raw + (sbase - smem_addr(smem_raw));
-    const uint32_t sQ = sbase + L::oQ, sK = sbase + L::oK, sV = sbase + L::oV;
-    const uint32_t bars = sbase + L::oBar;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + L::oBar + 8 * W_COUNT);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + L::oBar + 8 * W_COUNT + 8);
+    const uint32_t sQ = sbase + SM::oQ, sK = sbase + SM::oK, sV = sbase + SM::oV;
+    const uint32_t bars = sbase + SM::oBar;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + SM::oBar + 8 * W_COUNT);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + SM::oBar + 8 * W_COUNT + 8);
     auto bar = [&](int i) { return bars + 8u * i; };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pair = blockIdx.z * a.chunk + blockIdx.x;      // grid order as in the two-tile kernel
     if (pair >= a.b * a.nheads_grid) return;
-    const int b = pair / a.nheads_grid, h = pair % a.nheads_grid;
-    const int mblk = gridDim.y - 1 - blockIdx.y;
+    const int b = pair / a.nheads_grid, h = pair % a.nheads_grid;     // TREE: h is the KV head
+    const int split = TREE ? (int)blockIdx.y % a.nsplit : 0;
+    const int mblk = TREE ? (int)blockIdx.y / a.nsplit : (int)(gridDim.y - 1 - blockIdx.y);
     int q_off = 0, k_off = 0, sq = a.sq, sk = a.sk;
     if (a.cu_q) { q_off = a.cu_q[b]; sq = a.cu_q[b + 1] - q_off; k_off = a.cu_k[b]; sk = a.cu_k[b + 1] - k_off; }
-    if (a.seqused_k) sk = (int)max(0LL, min((long long)a.seqused_k[b] + a.s_new, (long long)a.sk));
-    const int m0 = mblk * 128;
-    if (m0 >= sq) return;
+    int L = 0;                                               // TREE: cached rows in front of the draft
+    if constexpr (TREE) {
+        L = tree_prefix(a.seqused_k, b, a.sk);
+        sk = (int)min((long long)L + sq, (long long)a.sk);
+    } else if (a.seqused_k) sk = (int)max(0LL, min((long long)a.seqused_k[b] + a.s_new, (long long)a.sk));
+    const int m0 = mblk * 128;                               // TREE: first stacked row
+    if (m0 >= (TREE ? sq * a.gq : sq)) return;
     if (g_fwd_sm100_error) return;
-    const int hk = h / (a.hq / a.hkv);
+    const int hk = TREE ? h : h / (a.hq / a.hkv);
     const int wl = a.wl, wr = a.causal ? 0 : a.wr;
-    const int rows = min(128, sq - m0);
+    const int rows = min(128, (TREE ? sq * a.gq : sq) - m0);
 
     int lo_first, hi_first, lo_last, hi_last;
     window_bounds(m0, sq, sk, wl, wr, lo_first, hi_first);
     window_bounds(m0 + rows - 1, sq, sk, wl, wr, lo_last, hi_last);
     int t_lo = lo_first / 128, t_hi = hi_last < 0 ? 0 : hi_last / 128 + 1;
     if (sk <= 0 || lo_first >= sk) { t_lo = 0; t_hi = 0; }
+    if constexpr (TREE) tree_split_tiles(tree_first_any(a.tree, L), sk, a.nsplit, split, a.min_split_keys, t_lo, t_hi);
     const int ntiles = max(0, t_hi - t_lo);
 
-    T* obase = reinterpret_cast<T*>(a.o) + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(q_off + m0) * a.o_ss + (int64_t)h * a.o_sh;
-    float* lbase = a.lse ? a.lse + (a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)h * a.lse_sh + (int64_t)(q_off + m0) * a.lse_ss : nullptr;
+    // output row, LSE slot and row in the partial buffers of tile row t
+    auto out_row = [&](int t) -> T* {
+        if constexpr (TREE) return reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_sb + (int64_t)((m0 + t) / a.gq) * a.o_ss + (int64_t)(hk * a.gq + (m0 + t) % a.gq) * a.o_sh;
+        else return reinterpret_cast<T*>(a.o) + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(q_off + m0 + t) * a.o_ss + (int64_t)h * a.o_sh;
+    };
+    auto lse_slot = [&](int t) -> float* {
+        if constexpr (TREE) return a.lse + (int64_t)b * a.lse_sb + (int64_t)(hk * a.gq + (m0 + t) % a.gq) * a.lse_sh + (int64_t)((m0 + t) / a.gq) * a.lse_ss;
+        else return a.lse + (a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)h * a.lse_sh + (int64_t)(q_off + m0 + t) * a.lse_ss;
+    };
+    auto part_row = [&](int t) -> int64_t {
+        return (int64_t)split * a.rows_all + ((int64_t)b * a.sq + (m0 + t) / a.gq) * a.hq + hk * a.gq + (m0 + t) % a.gq;
+    };
 
+    if (TREE && ntiles == 0 && a.nsplit > 1) {               // an empty split
+        if (tid < rows) a.lse_part[part_row(tid)] = -INFINITY;
+        return;
+    }
     if (ntiles == 0) {
         if (tid < rows) {
             uint4 z = make_uint4(0, 0, 0, 0);
-            T* orow = obase + (int64_t)tid * a.o_ss;
+            T* orow = out_row(tid);
 #pragma unroll
             for (int c = 0; c < D / 8; ++c)
                 if (c * 8 < a.d) reinterpret_cast<uint4*>(orow)[c] = z;
-            if (lbase) lbase[(int64_t)tid * a.lse_ss] = INFINITY;
+            if (a.lse) *lse_slot(tid) = INFINITY;
         }
         return;
     }
@@ -669,12 +746,32 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
     static_assert(128 * 56 + 256 * 224 <= 384 * 168, "register split exceeds the CTA's allocation");
     if (warp >= 8) {
     reg_dealloc<56>();
-    if (warp == 8) {
+    if (TREE && warp == 8) {
+        if (lane == 0) {
+            mbar_expect_tx(bar(W_Q), SM::kTile);
+#pragma unroll
+            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * SM::kSub, &a.tq, bar(W_Q), s * 64, hk, m0, b);
+        }
+        bool ok = true;                                      // the whole warp, one lane a box; order of the requests as below
+        for (int j = 0; j <= ntiles && ok; ++j) {
+            if (j < ntiles) {
+                if (j > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(W_KE), (j - 1) & 1, abort_flag, err, 1));
+                if (!ok) break;
+                tree_load_tile<NSUB>(a, &a.tk, sK, bar(W_KF), (t_lo + j) * 128, hk, b, lane);
+            }
+            const int jv = j == 0 ? 0 : j - 1;
+            if (j == 0 || j >= 2) {
+                if (jv >= 1) ok = __all_sync(0xffffffffu, mbar_wait(bar(W_VE), (jv - 1) & 1, abort_flag, err, 2));
+                if (!ok) break;
+                tree_load_tile<NSUB>(a, &a.tv, sV, bar(W_VF), (t_lo + jv) * 128, hk, b, lane);
+            }
+        }
+    } else if (warp == 8) {
         if (lane == 0) {
             tma_prefetch_desc(&a.tq); tma_prefetch_desc(&a.tk); tma_prefetch_desc(&a.tv);
-            mbar_expect_tx(bar(W_Q), L::kTile);
+            mbar_expect_tx(bar(W_Q), SM::kTile);
 #pragma unroll
-            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * L::kSub, &a.tq, bar(W_Q), s * 64, h, qrow0, qb);
+            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * SM::kSub, &a.tq, bar(W_Q), s * 64, h, qrow0, qb);
             const int32_t* btab = a.block_table ? a.block_table + (int64_t)b * a.bt_stride : nullptr;
             const int kbatch = a.cu_q ? 0 : (a.cache_batch_idx ? a.cache_batch_idx[b] : b);
             // where key tile j lives: (row, outermost coordinate), second half of the tile when it is copied in two boxes
@@ -694,11 +791,11 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
             auto load = [&](const CUtensorMap* map, uint32_t dst, int full_bar, int j) {
                 int krow, kouter, krow2, kouter2;
                 place(j, krow, kouter, krow2, kouter2);
-                mbar_expect_tx(bar(full_bar), L::kTile);
+                mbar_expect_tx(bar(full_bar), SM::kTile);
 #pragma unroll
                 for (int s = 0; s < NSUB; ++s) {
-                    tma_load_4d(dst + s * L::kSub, map, bar(full_bar), s * 64, hk, krow, kouter);
-                    if (a.kv_box == 64) tma_load_4d(dst + s * L::kSub + 64 * 128, map, bar(full_bar), s * 64, hk, krow2, kouter2);
+                    tma_load_4d(dst + s * SM::kSub, map, bar(full_bar), s * 64, hk, krow, kouter);
+                    if (a.kv_box == 64) tma_load_4d(dst + s * SM::kSub + 64 * 128, map, bar(full_bar), s * 64, hk, krow2, kouter2);
                 }
             };
             // order of the requests: K(0) V(0) K(1) | K(2) V(1) | K(3) V(2) ...: K(j) follows the scores of tile j - 1,
@@ -719,11 +816,11 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
             }
         }
     } else if (warp == 9) {
-        const uint64_t dQ = umma_desc(sQ, 16, 1024), dK = umma_desc(sK, 16, 1024), dV = umma_desc(sV, L::kSub, 1024);
+        const uint64_t dQ = umma_desc(sQ, 16, 1024), dK = umma_desc(sK, 16, 1024), dV = umma_desc(sV, SM::kSub, 1024);
         auto issue_qk = [&](int j) {
             const uint32_t d_s = tmem + (j & 1) * 128;
             static_for<0, NSUB>([&](auto sub) {
-                constexpr uint32_t o = sub.value * (L::kSub >> 4);
+                constexpr uint32_t o = sub.value * (SM::kSub >> 4);
                 umma_ss_group4<o, o + 2, o + 4, o + 6, o, o + 2, o + 4, o + 6>(d_s, dQ, dK, IDESC_QK, sub.value > 0);
             });
             umma_commit_w(bar(W_S0 + (j & 1)));
@@ -741,14 +838,15 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
             }
             ok = mbar_wait(bar(W_VF), j & 1, abort_flag, err, 6);
             if (!ok) break;
-            if (a.seqused_k && (t_lo + j) * 128 + 128 > sk) {
+            if constexpr (TREE) tree_clear_rows<NSUB>(a, sgen + SM::oV, (t_lo + j) * 128, L, b, lane);
+            else if (a.seqused_k && (t_lo + j) * 128 + 128 > sk) {
                 // stale cache rows past the sequence may hold NaN patterns: 0 x NaN is NaN, so the V rows are cleared
                 const int first = max(0, sk - (t_lo + j) * 128);
                 const int last = a.block_table ? 128 : min(128, a.sk - (t_lo + j) * 128);     // rows the copy fetched
 #pragma unroll
                 for (int sub = 0; sub < NSUB; ++sub)
                     for (int idx = first * 8 + lane; idx < last * 8; idx += 32)
-                        *reinterpret_cast<uint4*>(sgen + L::oV + sub * L::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(sgen + SM::oV + sub * SM::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async_smem();
                 __syncwarp();
             }
@@ -772,12 +870,25 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
         const int r = tid & 127;
         const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t t_o = tmem + lane_base + COL_O;
-        const int qi = m0 + r;
+        const int qi = TREE ? (m0 + r) / a.gq : m0 + r;
         int klo = 1, khi = 0;
-        if (r < rows) window_bounds(qi, sq, sk, wl, wr, klo, khi);
         int lo_l, hi_f, tmp;
-        window_bounds(m0, sq, sk, wl, wr, tmp, hi_f);
-        window_bounds(m0 + rows - 1, sq, sk, wl, wr, lo_l, tmp);
+        const uint32_t* tree_row = nullptr;
+        bool there = true;                                   // TREE, as in the two-tile kernel
+        if constexpr (TREE) {
+            klo = 0x7fffffff;
+            if (r < rows) {
+                klo = tree_first_key(a.tree, b, qi, L);
+                tree_row = a.tree.bits + (int64_t)(b * a.tree.tokens + qi) * a.tree.words;
+            }
+            there = klo != 0x7fffffff;
+            lo_l = tree_first_all(a.tree, L);
+            hi_f = L - 1;
+        } else {
+            if (r < rows) window_bounds(qi, sq, sk, wl, wr, klo, khi);
+            window_bounds(m0, sq, sk, wl, wr, tmp, hi_f);
+            window_bounds(m0 + rows - 1, sq, sk, wl, wr, lo_l, tmp);
+        }
         float m_used = -INFINITY, l_run = 0.f;
         const float sc = BIAS ? 1.f : a.scale_log2;
         const float cap_out = a.softcap * kLog2e;
@@ -821,10 +932,12 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
                 if (!full) {
 #pragma unroll
                     for (int c = 2 * hh; c < 2 * hh + 2; ++c) {
+                        uint32_t vis = 0;
+                        if constexpr (TREE) vis = there ? tree_visible32(a.tree, tree_row, n0 + c * 32, klo, L) : 0u;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const int col = n0 + c * 32 + i;
-                            if (col < klo || col > khi) sreg[c][i] = 0xff800000u;     // -inf
+                            if (TREE ? !(vis >> i & 1) : col < klo || col > khi) sreg[c][i] = 0xff800000u;     // -inf
                         }
                     }
                 }
@@ -892,16 +1005,30 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
             l_run += (sum_a.x + sum_b.x) + (sum_a.y + sum_b.y);
         }
         if (ok) ok = mbar_wait(bar(W_O), 0, abort_flag, err, 10);
+        if (TREE && !there) l_run = 0.f;
         if (ok) {
             tc_fence_after();
             const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-            T* orow = obase + (int64_t)r * a.o_ss;
+            T* orow = out_row(r);
+            float* prow = TREE && a.nsplit > 1 ? a.o_part + part_row(r) * a.d : nullptr;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t oreg[32];
                 tmem_ld32(t_o + c * 32, oreg);
                 tmem_wait_ld();
-                if (r < rows) {
+                if constexpr (TREE) {
+                    if (!there) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) oreg[i] = 0u;
+                    }
+                }
+                if (TREE && r < rows && prow) {
+#pragma unroll
+                    for (int v = 0; v < 8; ++v)
+                        if (c * 32 + v * 4 < a.d)
+                            reinterpret_cast<float4*>(prow + c * 32)[v] = make_float4(__uint_as_float(oreg[4 * v]) * inv, __uint_as_float(oreg[4 * v + 1]) * inv,
+                                                                                     __uint_as_float(oreg[4 * v + 2]) * inv, __uint_as_float(oreg[4 * v + 3]) * inv);
+                } else if (r < rows) {
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
                         uint4 pk;
@@ -913,7 +1040,8 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
                     }
                 }
             }
-            if (r < rows && lbase) lbase[(int64_t)r * a.lse_ss] = l_run > 0.f ? (m_used + log2f(l_run)) * kLn2 : INFINITY;
+            if (TREE && r < rows && prow) a.lse_part[part_row(r)] = l_run > 0.f ? (m_used + log2f(l_run)) * kLn2 : -INFINITY;
+            else if (r < rows && a.lse) *lse_slot(r) = l_run > 0.f ? (m_used + log2f(l_run)) * kLn2 : INFINITY;
         }
     }
     }
@@ -1024,15 +1152,16 @@ int grid_chunk(int64_t pairs, int64_t bytes_per_pair) {
     return (int)(c < 1 ? 1 : c);
 }
 
-template <typename T, int D, bool BIAS, bool DUAL>
+template <typename T, int D, bool BIAS, bool DUAL, bool TREE>
 static int launch_sm100_b(const fa_fwd_params& p, Sm100FwdArgs& a) {
     cudaStream_t st = reinterpret_cast<cudaStream_t>(p.stream);
-    auto kern = fwd_sm100_kernel2<T, D, BIAS, DUAL>;
+    auto kern = fwd_sm100_kernel2<T, D, BIAS, DUAL, TREE>;
     const int smem = FwdSm100Smem2<D, DUAL>::kBytes + 1024;
     if (int e = cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return e;
     const int qpc = 256 / a.gq;                              // query positions of a CTA
-    const unsigned nbx = (unsigned)(((p.sq + qpc - 1) / qpc) * a.nsplit);
-    a.nheads_grid = a.gq > 1 ? p.hkv : p.hq;
+    const int tree_rows = DUAL ? 128 : 256;
+    const unsigned nbx = (unsigned)((TREE ? (p.sq * a.gq + tree_rows - 1) / tree_rows : (p.sq + qpc - 1) / qpc) * a.nsplit);
+    a.nheads_grid = TREE || a.gq > 1 ? p.hkv : p.hq;
     a.chunk = grid_chunk((int64_t)p.b * a.nheads_grid, (int64_t)p.sk * p.d * 4);
     dim3 grid(a.chunk, nbx, (unsigned)(((int64_t)p.b * a.nheads_grid + a.chunk - 1) / a.chunk));
     kern<<<grid, 384, smem, st>>>(a);
@@ -1045,25 +1174,79 @@ static bool short_queries(const fa_fwd_params& p, int gq) { return (long)p.sq * 
 template <typename T, int D>
 static int launch_sm100_t(const fa_fwd_params& p, Sm100FwdArgs& a) {
     const bool bias = p.softcap > 0.f || p.alibi_slopes;
-    if (short_queries(p, a.gq)) return bias ? launch_sm100_b<T, D, true, true>(p, a) : launch_sm100_b<T, D, false, true>(p, a);
-    return bias ? launch_sm100_b<T, D, true, false>(p, a) : launch_sm100_b<T, D, false, false>(p, a);
+    if (short_queries(p, a.gq)) return bias ? launch_sm100_b<T, D, true, true, false>(p, a) : launch_sm100_b<T, D, false, true, false>(p, a);
+    return bias ? launch_sm100_b<T, D, true, false, false>(p, a) : launch_sm100_b<T, D, false, false, false>(p, a);
 }
-template <typename T, int D, bool BIAS>
+template <typename T, int D, bool BIAS, bool TREE>
 static int launch_sm100_wide_b(const fa_fwd_params& p, Sm100FwdArgs& a) {
     cudaStream_t st = reinterpret_cast<cudaStream_t>(p.stream);
-    auto kern = fwd_sm100_kernel_wide<T, D, BIAS>;
+    auto kern = fwd_sm100_kernel_wide<T, D, BIAS, TREE>;
     const int smem = FwdSm100SmemWide<D>::kBytes + 1024;
     if (int e = cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return e;
-    a.nheads_grid = p.hq;
-    a.chunk = grid_chunk((int64_t)p.b * p.hq, (int64_t)p.sk * p.d * 4);
-    dim3 grid(a.chunk, (p.sq + 127) / 128, (unsigned)(((int64_t)p.b * p.hq + a.chunk - 1) / a.chunk));
+    a.nheads_grid = TREE ? p.hkv : p.hq;
+    a.chunk = grid_chunk((int64_t)p.b * a.nheads_grid, (int64_t)p.sk * p.d * 4);
+    const unsigned blocks = TREE ? (unsigned)((p.sq * a.gq + 127) / 128 * a.nsplit) : (unsigned)((p.sq + 127) / 128);
+    dim3 grid(a.chunk, blocks, (unsigned)(((int64_t)p.b * a.nheads_grid + a.chunk - 1) / a.chunk));
     kern<<<grid, 384, smem, st>>>(a);
     mark_kernel(st);
     return cuda_ok(cudaGetLastError(), "fwd_sm100 launch");
 }
 template <typename T, int D>
 static int launch_sm100_wide_t(const fa_fwd_params& p, Sm100FwdArgs& a) {
-    return (p.softcap > 0.f || p.alibi_slopes) ? launch_sm100_wide_b<T, D, true>(p, a) : launch_sm100_wide_b<T, D, false>(p, a);
+    return (p.softcap > 0.f || p.alibi_slopes) ? launch_sm100_wide_b<T, D, true, false>(p, a) : launch_sm100_wide_b<T, D, false, false>(p, a);
+}
+
+// ---- tree of drafted tokens ---------------------------------------------------------------------------------------
+// rows of one K / V copy: what divides both a page and a tile
+static int tree_box(const fa_fwd_params& p) {
+    int box = 128;
+    while (p.block_table && p.page_size % box) box /= 2;
+    return box;
+}
+bool fwd_sm100_tree_supported(const fa_fwd_params& p) {
+    if (kernel_policy() != 0) return false;
+    if (p.d != 64 && p.d != 128 && p.d != 192 && p.d != 256) return false;
+    if (tree_box(p) < 16 || p.kv_entries > (1 << 24) || !(p.scale > 0.f) || p.sk <= 0) return false;
+    for (const fa_tensor* t : {&p.k, &p.v})
+        if (t->stride_h <= 0 || t->stride_s <= 0 || t->stride_b <= 0) return false;
+    return encode_fn() != nullptr;
+}
+long fwd_sm100_tree_ctas(const fa_fwd_params& p) {
+    const long rows = (long)p.sq * (p.hq / p.hkv), tile = p.d > 128 || p.softcap > 0.f || rows <= 128 ? 128 : 256;
+    return (long)p.b * p.hkv * ((rows + tile - 1) / tile);
+}
+template <typename T>
+static int launch_tree_t(const fa_fwd_params& p, Sm100FwdArgs& a) {
+    const bool dual = p.sq * a.gq <= 128;
+    if (p.d == 256) return p.softcap > 0.f ? launch_sm100_wide_b<T, 256, true, true>(p, a) : launch_sm100_wide_b<T, 256, false, true>(p, a);
+    if (p.d == 192) return p.softcap > 0.f ? launch_sm100_wide_b<T, 192, true, true>(p, a) : launch_sm100_wide_b<T, 192, false, true>(p, a);
+    if (p.d == 128) return dual ? launch_sm100_b<T, 128, false, true, true>(p, a) : launch_sm100_b<T, 128, false, false, true>(p, a);
+    return dual ? launch_sm100_b<T, 64, false, true, true>(p, a) : launch_sm100_b<T, 64, false, false, true>(p, a);
+}
+int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, float* o_part, float* lse_part) {
+    Sm100FwdArgs a = {};
+    a.gq = p.hq / p.hkv;
+    a.nsplit = nsplit; a.min_split_keys = min_split_keys; a.o_part = o_part; a.lse_part = lse_part;
+    a.rows_all = (int64_t)p.b * p.sq * p.hq;
+    a.kv_box = tree_box(p);
+    a.tree = tree;
+    const int64_t rows = p.block_table ? p.page_size : p.sk;
+    if (int e = make_tile_map(&a.tq, p.dtype, p.q.ptr, p.d, p.hkv, (int64_t)p.sq * a.gq, p.b, p.q.stride_h, p.q.stride_s, p.q.stride_b, 128)) return e;
+    if (int e = make_tile_map(&a.tk, p.dtype, p.k.ptr, p.d, p.hkv, rows, (int)p.kv_entries, p.k.stride_h, p.k.stride_s, p.k.stride_b, a.kv_box)) return e;
+    if (int e = make_tile_map(&a.tv, p.dtype, p.v.ptr, p.d, p.hkv, rows, (int)p.kv_entries, p.v.stride_h, p.v.stride_s, p.v.stride_b, a.kv_box)) return e;
+    a.seqused_k = p.seqused_k; a.block_table = p.block_table; a.cache_batch_idx = p.cache_batch_idx;
+    a.bt_stride = p.block_table_stride; a.page_size = p.page_size;
+    a.o = p.o.ptr; a.lse = p.lse;
+    a.o_sb = p.o.stride_b; a.o_ss = p.o.stride_s; a.o_sh = p.o.stride_h;
+    a.lse_sb = p.lse_stride_b; a.lse_sh = p.lse_stride_h; a.lse_ss = p.lse_stride_s;
+    a.b = p.b; a.sq = p.sq; a.sk = p.sk; a.hq = p.hq; a.hkv = p.hkv; a.d = p.d;
+    a.scale_log2 = p.scale * kLog2e;
+    a.softcap = p.softcap; a.cap_in = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
+    a.wl = a.wr = -1;
+    const bool single = p.d <= 128 && p.softcap > 0.f;
+    note_kernel(p.d > 128 ? "sm100_tcgen05_wide" : "sm100_tcgen05_2q", single ? FORM_ONE_TILE : p.d <= 128 && p.sq * a.gq <= 128 ? FORM_SHORT_QUERIES : FORM_USUAL);
+    if (single) return launch_fwd_single_sm100(p, a, true);
+    return p.dtype == FA_F16 ? launch_tree_t<__half>(p, a) : launch_tree_t<__nv_bfloat16>(p, a);
 }
 
 // query group stacked into the tile rows of the two-tile kernel (dense q shorter than 128, power-of-two group)

@@ -4,6 +4,7 @@
 #include "fa_utils.cuh"
 #include "fa_internal.h"
 #include "sm100_ptx.cuh"
+#include "tree_mask.cuh"
 
 namespace fa {
 
@@ -39,10 +40,62 @@ struct alignas(64) Sm100FwdArgs {
     float* lse_part;                     // (nsplit, rows_all)
     int64_t rows_all;
     int chunk, nheads_grid;              // grid order, see the kernels: (batch entry, head) pairs a chunk; heads of the grid
+    // TREE instantiations: a tree of drafted tokens behind the cached rows (tree_mask.cuh).  tq covers the stacked copy of q,
+    // (dim, KV head, token x group, batch); rows of a tile are stacked rows, of which gq (any number) make a token.  Splits
+    // share out the rows that the sequence has (tree_split_tiles), min_split_keys at least.
+    TreeMask tree;
+    int min_split_keys;
 };
 
+// TREE: key tile at cache row `pos`, in boxes of kv_box rows (what divides a page), one lane a box.  A row past the table or
+// on a page that is not in the cache lies outside the map: zeros.  The whole warp calls it.
+template <int NSUB>
+__device__ __forceinline__ void tree_load_tile(const Sm100FwdArgs& a, const CUtensorMap* map, uint32_t dst, uint32_t full, int pos, int hk, int b, int lane) {
+    if (lane == 0) sm100::mbar_expect_tx(full, NSUB * 128 * 128);
+    __syncwarp();
+    if (lane < 128 / a.kv_box) {
+        const int row = pos + lane * a.kv_box;
+        int krow = row, kouter = a.cache_batch_idx ? a.cache_batch_idx[b] : b;
+        if (a.block_table) {
+            kouter = row < a.sk ? a.block_table[(int64_t)b * a.bt_stride + row / a.page_size] : -1;
+            krow = row % a.page_size;
+        }
+#pragma unroll
+        for (int s = 0; s < NSUB; ++s) sm100::tma_load_4d(dst + s * 128 * 128 + lane * a.kv_box * 128, map, full, s * 64, hk, krow, kouter);
+    }
+    __syncwarp();
+}
+// TREE: rows of the V tile at cache row n0 that no token sees may hold anything, NaN included, and 0 x NaN is NaN: rows in
+// front of every window, drafted tokens that are not there, rows behind the draft.  The whole warp calls it.
+template <int NSUB>
+__device__ __forceinline__ void tree_clear_rows(const Sm100FwdArgs& a, unsigned char* v, int n0, int L, int b, int lane) {
+    const int first = tree_first_any(a.tree, L);
+    if (n0 >= first && n0 + 128 <= L) return;
+    uint32_t gone[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int row = n0 + w * 32 + lane, s = row - L;
+        const bool seen = s < 0 ? row >= first : s < a.tree.tokens && (a.tree.keys[b * a.tree.words + (s >> 5)] >> (s & 31) & 1);
+        gone[w] = __ballot_sync(0xffffffffu, !seen);
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (!gone[w]) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int chunk = i * 32 + lane;                     // 16-byte chunks of rows 32 w .. 32 w + 31, eight a row whatever the swizzle
+            if (gone[w] >> (chunk >> 3) & 1) {
+#pragma unroll
+                for (int s = 0; s < NSUB; ++s) *reinterpret_cast<uint4*>(v + s * 128 * 128 + w * 4096 + chunk * 16) = make_uint4(0, 0, 0, 0);
+            }
+        }
+    }
+    sm100::fence_proxy_async_smem();
+    __syncwarp();
+}
+
 // capped scores, head dims up to 128: one query tile a CTA, two CTAs an SM (fwd_single_sm100.cu)
-int launch_fwd_single_sm100(const fa_fwd_params& p, Sm100FwdArgs& a);
+int launch_fwd_single_sm100(const fa_fwd_params& p, Sm100FwdArgs& a, bool tree = false);
 int fwd_single_error_flag(bool clear);
 
 }  // namespace fa

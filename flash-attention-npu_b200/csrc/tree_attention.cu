@@ -147,9 +147,11 @@ void plan_tree(const fa_fwd_params& p, TreePlan& plan) {
     const long rows = (long)p.sq * (p.hq / p.hkv);
     plan.words = (p.sq + 31) / 32;
     plan.min_keys = 512;
-    const long base = (long)p.b * p.hkv * ((rows + kGenericBM - 1) / kGenericBM);
+    plan.sm100 = fwd_sm100_tree_supported(p) ? 1 : 0;
+    const long base = plan.sm100 ? fwd_sm100_tree_ctas(p) : (long)p.b * p.hkv * ((rows + kGenericBM - 1) / kGenericBM);
     const long most = ((long)p.sk + plan.min_keys - 1) / plan.min_keys;
-    long n = p.num_splits > 0 ? p.num_splits : (4l * sm_count() + base - 1) / base;
+    const long waves = plan.sm100 ? 2 : 4;
+    long n = p.num_splits > 0 ? p.num_splits : (waves * sm_count() + base - 1) / base;
     if (n > most) n = most;
     if (n > 256) n = 256;
     if (n > 65535 / p.b) n = 65535 / p.b;
@@ -273,7 +275,9 @@ int run_tree(const fa_tree_params& t) {
     p.q.stride_b = p.hkv * rows * p.d;
     float* o_part = plan.nsplit > 1 ? reinterpret_cast<float*>(ws + plan.o) : nullptr;
     float* lse_part = plan.nsplit > 1 ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;
-    if (int e = launch_fwd_generic_tree(p, mask, plan.nsplit, plan.min_keys, o_part, lse_part)) return e;
+    const int e = plan.sm100 ? launch_fwd_sm100_tree(p, mask, plan.nsplit, plan.min_keys, o_part, lse_part)
+                             : launch_fwd_generic_tree(p, mask, plan.nsplit, plan.min_keys, o_part, lse_part);
+    if (e) return e;
     return plan.nsplit > 1 ? launch_fwd_combine(p, plan.nsplit, o_part, lse_part, 0) : FA_OK;
 }
 

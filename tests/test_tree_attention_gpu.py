@@ -289,3 +289,23 @@ def test_empty_calls():
 
 def test_depths_of_the_reference():
     assert depths([-1, 0, 0, 2, -2, 4, 5, 7]) == [0, 1, 1, 2, -1, -1, -1, -1]
+
+
+@pytest.mark.parametrize("d,softcap,page,hq,t,name,form", [
+    (128, 0.0, 64, 8, 16, "sm100_tcgen05_2q", 1), (64, 0.0, 16, 14, 40, "sm100_tcgen05_2q", 0), (128, 20.0, 0, 6, 9, "sm100_tcgen05_2q", 2),
+    (256, 0.0, 32, 4, 9, "sm100_tcgen05_wide", 0), (192, 5.0, 128, 4, 9, "sm100_tcgen05_wide", 0), (96, 0.0, 64, 4, 9, "generic_mma", 0),
+    (128, 0.0, 48, 8, 16, "sm100_tcgen05_2q", 1), (128, 0.0, 40, 8, 16, "generic_mma", 0)])
+def test_which_kernel_runs(d, softcap, page, hq, t, name, form):
+    check(make(torch.bfloat16, d, hq, 2, [150, 300], t, page, seed=d + page), softcap=softcap)
+    assert capi.last_kernel() == name and capi.lib.fa_debug_get(8) == form
+
+
+def test_the_general_kernels_agree():
+    c = make(torch.bfloat16, 128, 14, 2, [400, 77], 30, 64, seed=31, ragged=True, rotary="half", axes=3)
+    capi.lib.fa_set_kernel_policy(1)
+    try:
+        check(c)
+        assert capi.last_kernel() == "generic_mma"
+    finally:
+        capi.lib.fa_set_kernel_policy(0)
+    check(c)
