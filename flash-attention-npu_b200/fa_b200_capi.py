@@ -271,6 +271,12 @@ else:
         return torch.cuda.current_stream(device).cuda_stream
 
 
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    raw_stream_of = torch._C._cuda_getCurrentRawStream         # of a device number
+else:
+    def raw_stream_of(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -281,6 +287,25 @@ def launch(fn, buf, device):
     else:
         with torch.cuda.device(device):
             check(fn(buf))
+
+
+def launch_on(fn, buf, index):
+    """launch() for a device number."""
+    if _current_device() == index:
+        status = fn(buf)
+    else:
+        with torch.cuda.device(index):
+            status = fn(buf)
+    if status:
+        check(status)
+
+
+def cuda_index(t):
+    """Device number of a CUDA tensor; the checks of a call compare these, which costs a third of comparing devices."""
+    i = t.get_device()
+    if i < 0:
+        raise RuntimeError("expected CUDA tensors: this library has no CPU implementation")
+    return i
 
 
 _PLAIN = (torch.Tensor, torch.nn.Parameter)

@@ -167,113 +167,150 @@ def mla_decode(q_nope, q_rope, latent_i8, scales, rope, block_table, cache_seqle
     return [out, lse]
 
 
-def _in_place(t):
-    """An input as 16-byte loads can read it: itself, or a copy where its last dim is strided or its rows are not aligned."""
-    s = t.stride()
-    return t if s[-1] == 1 and t.data_ptr() % 16 == 0 and not any(x % 8 for x in s[:-1]) else t.contiguous() if s[-1] != 1 else t.clone(
-        memory_format=torch.contiguous_format)
+def _input(t):
+    """An input and the four leaves of its fa_tensor, as 16-byte loads can read it: a copy where its last dim is strided or its
+    rows are not aligned."""
+    s0, s1, s2, s3 = t.stride()
+    ptr = t.data_ptr()
+    if s3 != 1 or ptr & 15 or (s0 | s1 | s2) & 7:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, s1, s2, s3 = t.stride()
+        ptr = t.data_ptr()
+    return t, (ptr, s0, s1, s2)
 
 
-def _int32(name, t, shapes, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+def _wrong_tensor(name, t, dtype, index):
+    capi.cuda_index(t)
+    raise RuntimeError(f"{name} must have the dtype and the device of q")
+
+
+def _int32(name, t, index):
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
         raise RuntimeError(f"{name} must be an int32 tensor")
-    if t.device != device:
+    if t.get_device() != index:
+        capi.cuda_index(t)
         raise RuntimeError(f"{name} must be on the device of q")
-    if tuple(t.shape) not in shapes:
-        raise RuntimeError(f"{name} must have shape " + " or ".join(str(s) for s in shapes))
-    return t if t.dim() == 0 or t.stride(-1) == 1 else t.contiguous()
 
 
 def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cache_batch_idx, page_table, rotary_cos, rotary_sin,
                      rotary_positions, rotary_sections, rotary_sections_cyclic, rotary_interleaved, softmax_scale, window_size_left,
                      window_size_right, softcap, num_splits):
-    """Attention of drafted tokens over a cache (no counterpart in the reference) -> [out, softmax_lse (B,H,T)]."""
-    capi.require_cuda(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cache_batch_idx, page_table, rotary_cos, rotary_sin,
-                      rotary_positions)
-    if q.dim() != 4 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+    """Attention of drafted tokens over a cache (no counterpart in the reference) -> [out, softmax_lse (B,H,T)].
+    A small draft's kernels run 15 us: the checks below ask each tensor as little as they can."""
+    index, dtype = capi.cuda_index(q), q.dtype
+    cache_shape = k_cache.shape
+    if q.dim() != 4 or len(cache_shape) != 4 or v_cache.shape != cache_shape:
         raise RuntimeError("q must be (batch, tokens, nheads, headdim), k_cache and v_cache of one shape with four dimensions")
     batch, tokens, hq, d = q.shape
-    hkv, device = k_cache.shape[2], q.device
-    code = _v2._dtype_code(q)
+    entries, rows, hkv, d_cache = cache_shape
+    code = capi.DTYPES.get(dtype)
+    if code is None:
+        raise RuntimeError("FlashAttention only supports FP16 and BF16 data types")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k", k), ("v", v)):
-        if t is not None and (t.dtype != q.dtype or t.device != device):
-            raise RuntimeError(f"{name} must have the dtype and the device of q")
-    if k_cache.shape[3] != d or d % 8 != 0 or d > 256:
+        if t is not None and (t.dtype is not dtype or t.get_device() != index):
+            _wrong_tensor(name, t, dtype, index)
+    if d_cache != d or d % 8 != 0 or d > 256:
         raise RuntimeError("q and the cache must have the same head dimension, a multiple of 8 of at most 256")
     if hkv == 0 or hq % hkv != 0:
         raise RuntimeError("Number of heads in key/value must divide number of heads in query")
-    if k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1:
+    kc, vc = k_cache.stride(), v_cache.stride()
+    if kc[3] != 1 or vc[3] != 1:
         raise RuntimeError("k_cache and v_cache must have contiguous last dimension")
     if (k is None) != (v is None):
         raise RuntimeError("k and v must be passed together")
-    if k is not None and (tuple(k.shape) != (batch, tokens, hkv, d) or tuple(v.shape) != (batch, tokens, hkv, d)):
-        raise RuntimeError(f"k and v must have shape {(batch, tokens, hkv, d)}")
-    if window_size_right not in (-1, 0):
+    if window_size_right != -1 and window_size_right != 0:
         raise RuntimeError("a tree of tokens has no window to the right")
     if softcap < 0.0:
         raise RuntimeError("softcap must be non-negative (0.0 disables softcap)")
     if num_splits < 0:
         raise RuntimeError("num_splits must be >= 0")
-    cache_seqlens = _int32("cache_seqlens", cache_seqlens, [(batch,)], device)
-    tree_parents = _int32("tree_parents", tree_parents, [(batch, tokens), (tokens,)], device)
+    _int32("cache_seqlens", cache_seqlens, index)
+    if cache_seqlens.shape != (batch,):
+        raise RuntimeError(f"cache_seqlens must have shape {(batch,)}")
+    if not cache_seqlens.is_contiguous():
+        cache_seqlens = cache_seqlens.contiguous()
+    _int32("tree_parents", tree_parents, index)
+    shape = tree_parents.shape
+    if shape != (batch, tokens) and shape != (tokens,):
+        raise RuntimeError(f"tree_parents must have shape {(batch, tokens)} or {(tokens,)}")
+    if tree_parents.stride(-1) != 1:
+        tree_parents = tree_parents.contiguous()
+    parents_sb = tree_parents.stride(0) if len(shape) == 2 else 0
+    batch_idx = 0
     if page_table is not None:
         if cache_batch_idx is not None:
             raise RuntimeError("cache_batch_idx is not used with a paged cache")
-        page_table = _int32("page_table", page_table, [(batch, page_table.shape[-1])], device)
-        table, capacity = (page_table.data_ptr(), page_table.stride(0), k_cache.shape[1]), page_table.shape[1] * k_cache.shape[1]
+        _int32("page_table", page_table, index)
+        shape = page_table.shape
+        if len(shape) != 2 or shape[0] != batch:
+            raise RuntimeError(f"page_table must have shape {(batch, 'max_pages')}")
+        if page_table.stride(1) != 1:
+            page_table = page_table.contiguous()
+        table, capacity = (page_table.data_ptr(), page_table.stride(0), rows), shape[1] * rows
     else:
-        table, capacity = (0, 0, 0), k_cache.shape[1]
+        table, capacity = (0, 0, 0), rows
         if cache_batch_idx is not None:
-            cache_batch_idx = _int32("cache_batch_idx", cache_batch_idx, [(batch,)], device)
+            _int32("cache_batch_idx", cache_batch_idx, index)
+            if cache_batch_idx.shape != (batch,):
+                raise RuntimeError(f"cache_batch_idx must have shape {(batch,)}")
             cache_batch_idx = cache_batch_idx.contiguous()
-        elif k_cache.shape[0] < batch:
+            batch_idx = cache_batch_idx.data_ptr()
+        elif entries < batch:
             raise RuntimeError("the cache has fewer entries than the batch")
+    if capacity >= 2 ** 31:
+        raise RuntimeError("a sequence of the cache has at most 2^31 - 1 rows")
     rotary, positions, axes = (0, 0, 0, 0, 0), (0, 0, 0), (0, 1)
-    keep = []
+    keep = None
     if rotary_cos is None:
         if rotary_positions is not None or rotary_sections is not None:
             raise RuntimeError("rotary positions and sections need rotary_cos and rotary_sin")
     else:
         if k is None:
             raise RuntimeError("rotary embedding is only applied when k and v are passed in")
-        if rotary_sin is None or rotary_cos.dim() != 2 or rotary_cos.shape != rotary_sin.shape:
+        shape = rotary_cos.shape
+        if rotary_sin is None or len(shape) != 2 or rotary_sin.shape != shape:
             raise RuntimeError("rotary_cos and rotary_sin must both have shape (seqlen_ro, rotary_dim / 2)")
-        if rotary_cos.device != device or rotary_sin.device != device:
+        if rotary_cos.get_device() != index or rotary_sin.get_device() != index:
+            capi.require_cuda(rotary_cos, rotary_sin)
             raise RuntimeError("rotary_cos and rotary_sin must be on the device of q")
-        pairs = rotary_cos.shape[1]
-        if rotary_cos.shape[0] == 0 or not 0 < 2 * pairs <= d:
+        rows_ro, pairs = shape
+        if rows_ro == 0 or not 0 < 2 * pairs <= d:
             raise RuntimeError("rotary_dim must be positive and at most the head dimension, with one table row at least")
-        rc, rs = rotary_cos.to(q.dtype).contiguous(), rotary_sin.to(q.dtype).contiguous()
-        rotary = (rc.data_ptr(), rs.data_ptr(), 2 * pairs, int(rotary_interleaved), rc.shape[0])
-        axis, where, n = axis_pointer(pairs, rotary_sections, rotary_sections_cyclic)
-        axes = (where, n)
-        keep += [rc, rs, axis]
+        if rotary_cos.dtype is not dtype or not rotary_cos.is_contiguous():
+            rotary_cos = rotary_cos.to(dtype).contiguous()
+        if rotary_sin.dtype is not dtype or not rotary_sin.is_contiguous():
+            rotary_sin = rotary_sin.to(dtype).contiguous()
+        rotary = (rotary_cos.data_ptr(), rotary_sin.data_ptr(), 2 * pairs, 1 if rotary_interleaved else 0, rows_ro)
+        if rotary_sections is not None:
+            keep, where, n = axis_pointer(pairs, rotary_sections, rotary_sections_cyclic)
+            axes = (where, n)
         if rotary_positions is not None:
-            pos = check_positions(rotary_positions, n, (batch, tokens), device)
-            pos = pos if pos.stride(-1) == 1 else pos.contiguous()
-            positions = (pos.data_ptr(), pos.stride(0), pos.stride(1))
-            keep.append(pos)
-    out = torch.empty((batch, tokens, hq, d), dtype=q.dtype, device=device)
-    lse = torch.empty((batch, hq, tokens), dtype=torch.float32, device=device)
+            rotary_positions, st = check_positions(rotary_positions, axes[1], (batch, tokens), index)
+            positions = (rotary_positions.data_ptr(), st[0], st[1])
+    out = q.new_empty((batch, tokens, hq, d))
+    lse = q.new_empty((batch, hq, tokens), dtype=torch.float32)
+    if k is not None and (k.shape != (batch, tokens, hkv, d) or v.shape != (batch, tokens, hkv, d)):
+        raise RuntimeError(f"k and v must have shape {(batch, tokens, hkv, d)}")
     if batch == 0 or tokens == 0:
         return [out, lse]
-    if k_cache.numel() == 0:
+    if entries == 0 or capacity == 0:
         raise RuntimeError("the cache has no rows")
-    q = _in_place(q)
+    q, q_leaves = _input(q)
     new = _v2._NO_TENSOR + _v2._NO_TENSOR
     if k is not None:
-        k, v = _in_place(k), _in_place(v)
-        new = _v2._leaves(k) + _v2._leaves(v)
-    parents_sb = tree_parents.stride(0) if tree_parents.dim() == 2 else 0
+        k, new = _input(k)
+        v, v_leaves = _input(v)
+        new = new + v_leaves
     buf = capi.TREE_BLOCK.new(
-        *_v2._leaves(q), *_v2._leaves(k_cache), *_v2._leaves(v_cache), *_v2._leaves(out), lse.data_ptr(), *lse.stride(),
-        0, 0, cache_seqlens.data_ptr(), *table, 0 if cache_batch_idx is None else cache_batch_idx.data_ptr(), 0, 0,
+        *q_leaves, k_cache.data_ptr(), kc[0], kc[1], kc[2], v_cache.data_ptr(), vc[0], vc[1], vc[2],
+        out.data_ptr(), tokens * hq * d, hq * d, d, lse.data_ptr(), hq * tokens, tokens, 1,
+        0, 0, cache_seqlens.data_ptr(), *table, batch_idx, 0, 0,
         batch, tokens, capacity, 0, 0, hq, hkv, d, d, softmax_scale, softcap, 0, _v2._i32(window_size_left), -1, code,
-        *new, tokens, *rotary, num_splits, 0, 0, 0, 0, 0, 0, 0, 0, k_cache.shape[0], capi.raw_stream(device),
+        *new, tokens, *rotary, num_splits, 0, 0, 0, 0, 0, 0, 0, 0, entries, capi.raw_stream_of(index),
         tree_parents.data_ptr(), parents_sb, *positions, *axes)
     nbytes = capi._tree_bytes(buf)
-    ws = capi.workspace(nbytes, device)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
     capi.set_workspace(capi.TREE_BLOCK, buf, ws, nbytes, "fwd.")
-    capi.launch(capi._call_tree, buf, device)
+    capi.launch_on(capi._call_tree, buf, index)
     del keep
     return [out, lse]

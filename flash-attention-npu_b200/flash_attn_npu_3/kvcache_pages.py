@@ -15,94 +15,117 @@ _VIEW = struct.Struct("=Qqqqqiii4x")
 assert _VIEW.size == capi.C.sizeof(capi.CacheView)
 
 
-def _int32(name, t, shape, device=None):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+def _int32(name, t, dims, index):
+    """Checks of an int32 tensor -> its shape.  A small call's kernels run 2 to 10 us: tensors are asked as little as possible."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
         raise RuntimeError(f"{name} must be an int32 tensor")
-    if not t.is_cuda:
-        raise RuntimeError("expected CUDA tensors: this library has no CPU implementation")
-    if device is not None and t.device != device:
+    if t.get_device() != index:
+        capi.cuda_index(t)
         raise RuntimeError(f"{name} must be on the device of the other tensors")
-    if len(shape) != t.dim() or any(s is not None and s != n for s, n in zip(shape, t.shape)):
-        raise RuntimeError(f"{name} must have shape {tuple('any' if s is None else s for s in shape)}, not {tuple(t.shape)}")
-    return t
+    shape = t.shape
+    if len(shape) != dims:
+        raise RuntimeError(f"{name} must have shape with {dims} dimension{'s' if dims > 1 else ''}, not {tuple(shape)}")
+    return shape
 
 
-def _read(name, t, shape, device=None):
-    """An input: a copy where its last dimension is strided."""
-    t = _int32(name, t, shape, device)
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+def _row(name, t, n, index):
+    """An input (n,) -> a dense tensor."""
+    if _int32(name, t, 1, index)[0] != n:
+        raise RuntimeError(f"{name} must have shape {(n,)}, not {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _written(name, t, shape, device=None):
-    """A tensor that is changed in place."""
-    t = _int32(name, t, shape, device)
-    s = t.stride()
-    if (s[-1] != 1 and t.shape[-1] > 1) or (len(s) == 2 and t.shape[0] > 1 and s[0] < t.shape[1]):
+def _read_table(name, t, b, index):
+    """An input (b, any), b None: any -> (tensor, its shape, distance of its rows); a copy where its last dimension is strided."""
+    shape = _int32(name, t, 2, index)
+    if b is not None and shape[0] != b:
+        raise RuntimeError(f"{name} must have shape {(b, 'any')}, not {tuple(shape)}")
+    st = t.stride()
+    if st[1] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, shape, st[0]
+
+
+def _written_table(name, t, index):
+    """A table that is changed in place -> (b, width, distance of its rows)."""
+    b, width = _int32(name, t, 2, index)
+    s0, s1 = t.stride()
+    if (s1 != 1 and width > 1) or (b > 1 and s0 < width):
         raise RuntimeError(f"{name} is changed in place: its last dimension must be contiguous and its rows apart")
-    return t
+    return b, width, s0
+
+
+def _pool(page_refs):
+    """-> (device number, pages)"""
+    if not isinstance(page_refs, torch.Tensor):
+        raise RuntimeError("page_refs must be an int32 tensor")
+    index = capi.cuda_index(page_refs)
+    pages = _int32("page_refs", page_refs, 1, index)[0]
+    if not page_refs.is_contiguous():
+        raise RuntimeError("page_refs is changed in place: it must be contiguous")
+    if not 0 < pages <= 1 << 24:
+        raise RuntimeError("page_refs must have 1 to 2^24 entries")
+    return index, pages
 
 
 def _views(caches):
-    """Caches -> (packed fa_cache_view array, how many, entries, rows of one, device).  A tensor of up to four dimensions is one
-    cache (entries, rows, [heads,] [dim]); one of five is a stack of caches."""
-    caches = [caches] if isinstance(caches, torch.Tensor) else list(caches)
+    """Caches -> (packed fa_cache_view array, how many, entries, rows of one, device number).  A tensor of up to four dimensions
+    is one cache (entries, rows, [heads,] [dim]); one of five is a stack of caches."""
+    caches = (caches,) if isinstance(caches, torch.Tensor) else tuple(caches)
     if not caches:
         raise RuntimeError("at least one cache is needed")
-    entries = rows = device = None
-    buf = bytearray(_VIEW.size * len(caches))
-    for i, c in enumerate(caches):
-        if not isinstance(c, torch.Tensor) or not 2 <= c.dim() <= 5:
-            raise RuntimeError("a cache must be a tensor (num_pages, page_size, [nheads,] [headdim]), or a stack of such with five dimensions")
-        if not c.is_cuda:
-            raise RuntimeError("expected CUDA tensors: this library has no CPU implementation")
-        size, shape, st = c.element_size(), tuple(c.shape), c.stride()
+    pack, size_of = _VIEW.pack_into, _VIEW.size
+    buf = (capi.C.c_char * (size_of * len(caches)))()
+    entries = rows = index = None
+    at = 0
+    for c in caches:
+        if not isinstance(c, torch.Tensor):
+            raise RuntimeError("caches must be tensors")
+        shape, st, size = c.shape, c.stride(), c.element_size()
+        dims = len(shape)
         n, sc = 1, 0
-        if len(shape) == 5:
+        if dims == 5:
             n, sc = shape[0], st[0]
             shape, st = shape[1:], st[1:]
-        heads, sh, dim = (shape[2], st[2], shape[3]) if len(shape) == 4 else (1, 0, shape[2] if len(shape) == 3 else 1)
-        if len(shape) > 2 and st[-1] != 1:
+        elif not 2 <= dims <= 4:
+            raise RuntimeError("a cache must be a tensor (num_pages, page_size, [nheads,] [headdim]), or a stack of such with five dimensions")
+        heads, sh, dim = (shape[2], st[2], shape[3]) if dims >= 4 else (1, 0, shape[2] if dims == 3 else 1)
+        if dims > 2 and st[-1] != 1:
             raise RuntimeError("caches must have a contiguous last dimension")
-        if (n > 1 and sc == 0) or st[0] == 0 and shape[0] > 1 or st[1] == 0 and shape[1] > 1 or heads > 1 and sh == 0:
-            raise RuntimeError("caches may not be expanded")
-        if i == 0:
-            entries, rows, device = shape[0], shape[1], c.device
-        elif (shape[0], shape[1]) != (entries, rows) or c.device != device:
+        if index is None:
+            entries, rows, index = shape[0], shape[1], capi.cuda_index(c)
+        elif shape[0] != entries or shape[1] != rows or c.get_device() != index:
+            capi.cuda_index(c)
             raise RuntimeError("all caches must have the same number of pages, the same page size and the same device")
-        if c.numel() == 0:
+        if n * entries * rows * heads * dim == 0:
             raise RuntimeError("a cache is empty")
-        _VIEW.pack_into(buf, i * _VIEW.size, c.data_ptr(), sc * size, st[0] * size, st[1] * size, sh * size, n, heads, dim * size)
-    return buf, len(caches), entries, rows, device
+        if (n > 1 and sc == 0) or (st[0] == 0 and entries > 1) or (st[1] == 0 and rows > 1) or (heads > 1 and sh == 0):
+            raise RuntimeError("caches may not be expanded")
+        pack(buf, at, c.data_ptr(), sc * size, st[0] * size, st[1] * size, sh * size, n, heads, dim * size)
+        at += size_of
+    return buf, len(caches), entries, rows, index
 
 
-def _launch(fn, device, views=None, num_views=0, num_pages=0, page_size=0, refs=None, table=None, b=0, width=0, extra=0, n=0,
-            keep_parents=0, seqlens=None, rows=None, rows2=None, rows_stride=0, batch_idx=None, new_table=None, new_seqlens=None,
-            missing=None, workspace_rows=None):
-    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    ws, nbytes = None, 0
-    if workspace_rows is not None:
-        nbytes = capi.lib.fa_pages_workspace_bytes(workspace_rows, num_pages)
-        ws = capi.workspace(nbytes, device)
-    host = (capi.C.c_char * len(views)).from_buffer(views) if views is not None else None
-    buf = capi.PAGES_BLOCK.new(
-        0 if host is None else capi.C.addressof(host), num_views, num_pages, page_size, p(refs), p(table), 0 if table is None else table.stride(0),
-        b, width, extra, n, keep_parents, p(seqlens), p(rows), p(rows2), rows_stride, p(batch_idx), p(new_table), p(new_seqlens), p(missing),
-        p(ws), nbytes, capi.raw_stream(device))
-    capi.launch(fn, buf, device)
-
-
-def _extra(extra, page_size):
+def _sizes(extra, page_size):
     if type(extra) is not int or not 0 <= extra < 2 ** 31:
         raise RuntimeError("extra must be a non-negative integer")
     if type(page_size) is not int or not 0 < page_size < 2 ** 31:
         raise RuntimeError("page_size must be a positive integer")
 
 
-def _pool(page_refs):
-    refs = _written("page_refs", page_refs, (None,))
-    if not 0 < refs.shape[0] <= 1 << 24:
-        raise RuntimeError("page_refs must have 1 to 2^24 entries")
-    return refs
+def _run(fn, index, views, num_caches, num_pages, page_size, refs, table, table_stride, b, width, extra, n, keep_parents, seqlens, rows,
+         rows2, rows_stride, batch_idx, new_table, new_seqlens, missing, ws=None):
+    """The library call: tensors, or None, where the block takes pointers."""
+    p = [0 if t is None else t.data_ptr() for t in (refs, table, seqlens, rows, rows2, batch_idx, new_table, new_seqlens, missing, ws)]
+    buf = capi.PAGES_BLOCK.new(
+        0 if views is None else capi.C.addressof(views), num_caches, num_pages, page_size, p[0], p[1], table_stride, b, width, extra, n,
+        keep_parents, p[2], p[3], p[4], rows_stride, p[5], p[6], p[7], p[8], p[9], 0 if ws is None else ws.numel() * 4, capi.raw_stream_of(index))
+    capi.launch_on(fn, buf, index)
+
+
+def _workspace(like, rows, num_pages):
+    return like.new_empty((capi.lib.fa_pages_workspace_bytes(rows, num_pages) + 3) // 4)
 
 
 def kvcache_reserve(page_refs, page_table, cache_seqlens, page_size, extra=0):
@@ -110,14 +133,13 @@ def kvcache_reserve(page_refs, page_table, cache_seqlens, page_size, extra=0):
     -1 get the lowest free pages, rows in order and entries in order, with a count of 1.  cache_seqlens int32 (batch,).
     Rows that need more pages than the table is wide get what fits.  Returns `missing`, int32 (1,): entries that stayed -1
     because no page was free."""
-    refs = _pool(page_refs)
-    _extra(extra, page_size)
-    table = _written("page_table", page_table, (None, None), refs.device)
-    b, width = table.shape
-    lens = _read("cache_seqlens", cache_seqlens, (b,), refs.device)
-    missing = torch.empty((1,), dtype=torch.int32, device=refs.device)
-    _launch(capi._call_reserve, refs.device, num_pages=refs.shape[0], page_size=page_size, refs=refs, table=table, b=b, width=width,
-            extra=extra, seqlens=lens, missing=missing, workspace_rows=b)
+    index, pages = _pool(page_refs)
+    _sizes(extra, page_size)
+    b, width, stride = _written_table("page_table", page_table, index)
+    lens = _row("cache_seqlens", cache_seqlens, b, index)
+    missing = page_refs.new_empty(1)
+    _run(capi._call_reserve, index, None, 0, pages, page_size, page_refs, page_table, stride, b, width, extra, 0, 0, lens, None, None, 0, None,
+         None, None, missing, _workspace(page_refs, b, pages))
     return missing
 
 
@@ -125,15 +147,15 @@ def kvcache_free(page_refs, page_table, cache_seqlens: Optional[torch.Tensor] = 
     """Let go of the pages behind cache_seqlens + extra rows (of all pages when cache_seqlens is None; page_size is only needed
     with it), in place: their counts
     drop by one and their entries of page_table become -1.  A page whose count is 0 stays at 0."""
-    refs = _pool(page_refs)
+    index, pages = _pool(page_refs)
+    b, width, stride = _written_table("page_table", page_table, index)
     if cache_seqlens is None:
-        page_size, extra = 1, 0
-    _extra(extra, page_size)
-    table = _written("page_table", page_table, (None, None), refs.device)
-    b, width = table.shape
-    lens = None if cache_seqlens is None else _read("cache_seqlens", cache_seqlens, (b,), refs.device)
-    _launch(capi._call_free, refs.device, num_pages=refs.shape[0], page_size=page_size, refs=refs, table=table, b=b, width=width,
-            extra=extra, seqlens=lens)
+        page_size, extra, lens = 1, 0, None
+    else:
+        _sizes(extra, page_size)
+        lens = _row("cache_seqlens", cache_seqlens, b, index)
+    _run(capi._call_free, index, None, 0, pages, page_size, page_refs, page_table, stride, b, width, extra, 0, 0, lens, None, None, 0, None,
+         None, None, None)
 
 
 def kvcache_fork(caches, page_refs, page_table, cache_seqlens, parents, keep_parents=False):
@@ -149,30 +171,29 @@ def kvcache_fork(caches, page_refs, page_table, cache_seqlens, parents, keep_par
     dimensions, such as scales), or of five dimensions, a stack of such.  cache_seqlens int32 (batch,).
     Returns (page_table (n, max_pages), cache_seqlens (n,), missing (1,)): rows whose copy found no free page end with their
     last full page and are counted in `missing`."""
-    refs = _pool(page_refs)
-    views, num, pages, page_size, device = _views(caches)
-    if pages != refs.shape[0] or refs.device != device:
+    index, pages = _pool(page_refs)
+    views, num, entries, page_size, device = _views(caches)
+    if entries != pages or device != index:
         raise RuntimeError("page_refs must have one entry for every page of the caches, on their device")
-    table = _read("page_table", page_table, (None, None), device)
-    b, width = table.shape
-    lens = _read("cache_seqlens", cache_seqlens, (b,), device)
-    parents = _read("parents", parents, (None,), device)
-    n = parents.shape[0]
-    new_table = torch.empty((n, width), dtype=torch.int32, device=device)
-    new_lens = torch.empty((n,), dtype=torch.int32, device=device)
-    missing = torch.empty((1,), dtype=torch.int32, device=device)
-    _launch(capi._call_fork, device, views, num, pages, page_size, refs, table, b, width, 0, n, int(bool(keep_parents)), lens, parents,
-            new_table=new_table, new_seqlens=new_lens, missing=missing, workspace_rows=n)
+    table, (b, width), stride = _read_table("page_table", page_table, None, index)
+    lens = _row("cache_seqlens", cache_seqlens, b, index)
+    n = _int32("parents", parents, 1, index)[0]
+    if not parents.is_contiguous():
+        parents = parents.contiguous()
+    new_table = page_refs.new_empty((n, width))
+    new_lens, missing = page_refs.new_empty(n), page_refs.new_empty(1)
+    _run(capi._call_fork, index, views, num, pages, page_size, page_refs, table, stride, b, width, 0, n, 1 if keep_parents else 0, lens, parents,
+         None, 0, None, new_table, new_lens, missing, _workspace(page_refs, n, pages))
     return new_table, new_lens, missing
 
 
 def kvcache_copy_pages(caches, src, dst):
     """Copy page src[i] to page dst[i] (int32 (n,)) in all caches (as in kvcache_fork).  Pairs with a page outside the cache
     are skipped.  A page that is written may not stand anywhere else in the lists."""
-    views, num, pages, page_size, device = _views(caches)
-    src = _read("src", src, (None,), device)
-    dst = _read("dst", dst, (src.shape[0],), device)
-    _launch(capi._call_copy, device, views, num, pages, page_size, n=src.shape[0], rows=src, rows2=dst)
+    views, num, pages, page_size, index = _views(caches)
+    n = _int32("src", src, 1, index)[0]
+    src, dst = _row("src", src, n, index), _row("dst", dst, n, index)
+    _run(capi._call_copy, index, views, num, pages, page_size, None, None, 0, 0, 0, 0, n, 0, None, src, dst, 0, None, None, None, None)
 
 
 def kvcache_compact(caches, cache_seqlens, kept, counts: Optional[torch.Tensor] = None, page_table: Optional[torch.Tensor] = None,
@@ -185,24 +206,24 @@ def kvcache_compact(caches, cache_seqlens, kept, counts: Optional[torch.Tensor] 
     sequence's list ends at the first entry that is not larger than the one before, or negative, or past the capacity.  The
     rows that move must lie on pages that no other sequence holds; a row on a page that is not in the cache is left out of
     the move.  cache_seqlens of zeros prunes whole sequences.  Returns the new lengths, int32 (batch,)."""
-    views, num, pages, page_size, device = _views(caches)
-    lens = _read("cache_seqlens", cache_seqlens, (None,), device)
-    b = lens.shape[0]
-    kept = _read("kept", kept, (b, None), device)
-    counts = None if counts is None else _read("counts", counts, (b,), device)
-    table, width = None, 1
+    views, num, entries, rows, index = _views(caches)
+    b = _int32("cache_seqlens", cache_seqlens, 1, index)[0]
+    lens = cache_seqlens if cache_seqlens.is_contiguous() else cache_seqlens.contiguous()
+    kept, (_, n), kept_stride = _read_table("kept", kept, b, index)
+    if counts is not None:
+        counts = _row("counts", counts, b, index)
+    table, width, stride = None, 1, 0
     if page_table is not None:
         if cache_batch_idx is not None:
             raise RuntimeError("cache_batch_idx is not used with a paged cache")
-        table = _read("page_table", page_table, (b, None), device)
-        width = table.shape[1]
+        table, (_, width), stride = _read_table("page_table", page_table, b, index)
         if width == 0:
             raise RuntimeError("page_table has no entries")
     elif cache_batch_idx is not None:
-        cache_batch_idx = _read("cache_batch_idx", cache_batch_idx, (b,), device)
-    elif pages < b:
+        cache_batch_idx = _row("cache_batch_idx", cache_batch_idx, b, index)
+    elif entries < b:
         raise RuntimeError("the caches have fewer entries than the batch")
-    out = torch.empty((b,), dtype=torch.int32, device=device)
-    _launch(capi._call_compact, device, views, num, pages, page_size, table=table, b=b, width=width, n=kept.shape[1], seqlens=lens,
-            rows=kept, rows2=counts, rows_stride=kept.stride(0), batch_idx=cache_batch_idx, new_seqlens=out)
+    out = lens.new_empty(b)
+    _run(capi._call_compact, index, views, num, entries, rows, None, table, stride, b, width, 0, n, 0, lens, kept, counts, kept_stride,
+         cache_batch_idx, None, out, None)
     return out

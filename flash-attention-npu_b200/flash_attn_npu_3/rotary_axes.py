@@ -37,54 +37,73 @@ def axis_pointer(pairs, sections, cyclic):
     return table, ctypes.addressof(table), len(sections)
 
 
-def check_positions(positions, axes, lead, device):
-    """positions (axes, *lead) int32, or (*lead) for one axis -> a tensor (axes, *lead)."""
-    if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int32:
+def check_positions(positions, axes, lead, index):
+    """positions (axes, *lead) int32, or (*lead) for one axis -> (a tensor with a dense last dim, its strides as of (axes, *lead))."""
+    if not isinstance(positions, torch.Tensor) or positions.dtype is not torch.int32:
         raise RuntimeError("positions must be an int32 tensor")
-    if positions.device != device:
+    if positions.get_device() != index:
+        capi.cuda_index(positions)
         raise RuntimeError("positions must be on the device of the tensors that they belong to")
-    shape = tuple(positions.shape)
-    if axes == 1 and shape == lead:
-        positions = positions.unsqueeze(0)
-    elif shape != (axes, *lead):
-        raise RuntimeError(f"positions must have shape {(axes, *lead)}" + (f" or {lead}" if axes == 1 else ""))
-    return positions if positions.stride(-1) == 1 or positions.shape[-1] == 1 else positions.contiguous()
+    shape = positions.shape
+    one = axes == 1 and shape == lead
+    if not one and shape != (axes, *lead):
+        raise RuntimeError(f"positions must have shape {(axes, *lead)}" + (f" or {tuple(lead)}" if axes == 1 else ""))
+    st = positions.stride()
+    if st[-1] != 1:
+        positions = positions.contiguous()
+        st = positions.stride()
+    return positions, (0,) + st if one else st
 
 
 _NONE = (0, 0, 0, 0)
 
 
-def _leaves(t):
+def _leaves(t, st):
     """The four leaves of an fa_tensor of (B, S, H, D), or of packed (T, H, D) as one batch entry."""
-    s = t.stride()
-    return (t.data_ptr(), s[0], s[1], s[2]) if len(s) == 4 else (t.data_ptr(), 0, s[0], s[1])
+    return (t.data_ptr(), st[0], st[1], st[2]) if len(st) == 4 else (t.data_ptr(), 0, st[0], st[1])
 
 
-def _run(q, k, q_out, k_out, cos, sin, positions, sections, cyclic, interleaved, backward):
-    """The library call; everything has been checked, positions is (axes, *lead)."""
-    pairs = cos.shape[1]
+def _run(q, k, cos, sin, positions, sections, cyclic, interleaved, backward, inplace):
+    """The library call; everything has been checked.  positions (axes, *lead), or (*lead) for one axis."""
+    rows, pairs = cos.shape
     keep, axis, axes = axis_pointer(pairs, sections, cyclic)
-    packed = q.dim() == 3
-    b, s = (1, q.shape[0]) if packed else q.shape[:2]
+    shape, st = q.shape, q.stride()
+    if st[-1] != 1:
+        q = q.contiguous()
+        st = q.stride()
+    packed = len(shape) == 3
+    b, s = (1, shape[0]) if packed else (shape[0], shape[1])
+    hq, d = shape[-2], shape[-1]
     pos = positions.stride()
-    d = q.shape[-1]
-    if q.numel() == 0 and (k is None or k.numel() == 0):
-        return
-    buf = capi.ROTARY_BLOCK.new(
-        *_leaves(q), *(_NONE if k is None else _leaves(k)), *_leaves(q_out), *(_NONE if k is None else _leaves(k_out)),
-        cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), pos[0], 0 if packed else pos[1], axis, axes, b, s,
-        q.shape[-2], 0 if k is None else k.shape[-2], d, 2 * pairs, int(interleaved), cos.shape[0], int(backward),
-        capi.DTYPES[q.dtype], 2 if cos.dtype == torch.float32 else capi.DTYPES[cos.dtype], capi.raw_stream(q.device))
-    capi.launch(capi._call_rotary, buf, q.device)
+    if len(pos) == len(shape) - 2:
+        pos = (0,) + pos
+    q_out = q if inplace else q.new_empty(shape)
+    dense = (s * hq * d, hq * d, d)
+    q_in = _leaves(q, st)
+    q_to = q_in if inplace else (q_out.data_ptr(),) + dense
+    k_out, hk, k_in, k_to = None, 0, _NONE, _NONE
+    if k is not None:
+        st = k.stride()
+        if st[-1] != 1:
+            k = k.contiguous()
+            st = k.stride()
+        hk = k.shape[-2]
+        k_out = k if inplace else k.new_empty(k.shape)
+        k_in = _leaves(k, st)
+        k_to = k_in if inplace else (k_out.data_ptr(), s * hk * d, hk * d, d)
+    if b * s * (hq + hk) > 0:
+        index = q.get_device()
+        buf = capi.ROTARY_BLOCK.new(
+            *q_in, *k_in, *q_to, *k_to, cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), pos[0], 0 if packed else pos[1],
+            axis, axes, b, s, hq, hk, d, 2 * pairs, 1 if interleaved else 0, rows, 1 if backward else 0,
+            capi.DTYPES[q.dtype], 2 if cos.dtype is torch.float32 else capi.DTYPES[cos.dtype], capi.raw_stream_of(index))
+        capi.launch_on(capi._call_rotary, buf, index)
     del keep
+    return q_out, k_out
 
 
 def _out_of_place(q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
-    q, k = (x.contiguous() if x is not None and x.stride(-1) != 1 else x for x in (q, k))
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    _run(q, k, q_out, k_out, cos, sin, positions, sections, cyclic, interleaved, backward)
-    return q_out, k_out
+    return _run(q, k, cos, sin, positions, sections, cyclic, interleaved, backward, False)
 
 
 @torch.library.custom_op("flash_attn_npu_3::_rotary_axes", mutates_args=(), device_types="cuda")
@@ -149,26 +168,35 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
 
     inplace writes into q and k instead of new tensors (only where no gradient is needed).
     Returns (q, k), or q alone when k is None."""
-    capi.require_cuda(q, k, cos, sin, positions)
-    if q.dtype not in capi.DTYPES or (k is not None and k.dtype != q.dtype):
+    index, dtype, shape = capi.cuda_index(q), q.dtype, q.shape
+    if dtype not in capi.DTYPES or (k is not None and k.dtype is not dtype):
         raise RuntimeError("rotary embedding only supports FP16 and BF16 data types, the same for q and k")
-    if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
-        raise RuntimeError("q must be (batch, seqlen, nheads, headdim) or (total, nheads, headdim), and k the same but for its heads")
-    device = q.device
-    if any(t is not None and t.device != device for t in (k, cos, sin)):
-        raise RuntimeError("q, k, cos and sin must be on one device")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.dtype not in (q.dtype, torch.float32):
+    n = len(shape)
+    if n != 3 and n != 4:
+        raise RuntimeError("q must be (batch, seqlen, nheads, headdim) or (total, nheads, headdim)")
+    lead = shape[:-2]
+    if k is not None:
+        other = k.shape
+        if len(other) != n or other[:-2] != lead or other[-1] != shape[-1]:
+            raise RuntimeError("k must have the shape of q but for its heads")
+    for t in (k, cos, sin):
+        if t is not None and t.get_device() != index:
+            capi.cuda_index(t)
+            raise RuntimeError("q, k, cos and sin must be on one device")
+    table = cos.shape
+    if len(table) != 2 or sin.shape != table or sin.dtype is not cos.dtype or (cos.dtype is not dtype and cos.dtype is not torch.float32):
         raise RuntimeError("cos and sin must both have shape (seqlen_ro, rotary_dim / 2), in q's dtype or fp32")
-    d, pairs = q.shape[-1], cos.shape[1]
-    if d > 256 or d % 2 or not 0 < 2 * pairs <= d or cos.shape[0] == 0:
+    d, (rows, pairs) = shape[-1], table
+    if d > 256 or d % 2 or not 0 < 2 * pairs <= d or rows == 0:
         raise RuntimeError("the head dimension must be even and at most 256, rotary_dim positive and at most that, with one table row at least")
+    sections_cyclic = bool(sections_cyclic)
     if sections is not None:
         sections = list(sections)
-        axis_table(pairs, tuple(sections), bool(sections_cyclic))
-    positions = check_positions(positions, 1 if sections is None else len(sections), tuple(q.shape[:-2]), device)
+        axis_table(pairs, tuple(sections), sections_cyclic)
+    positions, _ = check_positions(positions, 1 if sections is None else len(sections), lead, index)
     if not cos.is_contiguous() or not sin.is_contiguous():
         cos, sin = cos.contiguous(), sin.contiguous()
-    args = (cos, sin, positions, sections, bool(sections_cyclic), bool(interleaved))
+    args = (cos, sin, positions, sections, sections_cyclic, bool(interleaved))
     if inplace:
         for t in (q, k):
             if t is None:
@@ -177,7 +205,7 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
                 raise RuntimeError("inplace rotary embedding is not differentiable: detach q and k, or leave inplace out")
             if t.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise RuntimeError("inplace rotary embedding needs a contiguous last dimension and no expanded dimensions")
-        _run(q, k, q, k, *args, False)
+        _run(q, k, *args, False, True)
     else:
         q, k = _apply(q, k, *args, False)
     return q if k is None else (q, k)
