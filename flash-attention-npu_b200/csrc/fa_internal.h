@@ -7,6 +7,22 @@
 
 namespace fa {
 
+// Launch of a kernel that may start before the one in front of it on the stream has finished (grid_wait_for_previous() in it)
+template <typename Kernel, typename Arg>
+inline cudaError_t launch_early(Kernel kernel, dim3 grid, int threads, size_t smem, cudaStream_t st, const Arg& arg) {
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, arg);
+}
+
 // error reporting (thread-local message, see fa_api.cu)
 int fail(int code, const char* fmt, ...);
 // The name that fa_last_kernel() reports, and which form of that kernel ran (fa_debug_get key 8): several forms share a name
@@ -48,7 +64,8 @@ int launch_fwd_generic(const fa_fwd_params& p, const FwdPlan& plan, float* o_par
 struct TreeMask;                                     // tree_mask.cuh
 bool fwd_sm100_tree_supported(const fa_fwd_params& p);
 long fwd_sm100_tree_ctas(const fa_fwd_params& p);     // CTAs of one key split
-int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, float* o_part, float* lse_part);
+bool fwd_sm100_tree_shared(const fa_fwd_params& p);  // runs on the kernel that shares out the key tiles itself: no splits
+int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, int shares, float* o_part, float* lse_part);
 int launch_fwd_generic_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, float* o_part, float* lse_part);
 int launch_fwd_decode(const fa_fwd_params& p, const FwdPlan& plan, float* o_part, float* lse_part);
 bool fwd_decode_supported(const fa_fwd_params& p);

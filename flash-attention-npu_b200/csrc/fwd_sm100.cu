@@ -31,8 +31,6 @@ __device__ int g_fwd_sm100_error = 0;
 // groups and both accumulators work on the SAME rows, group A on the even key tiles and group B on the odd ones, and the two
 // partial results are merged in the epilogue.  With one tile in flight the K and V stream stood still while that tile went
 // through QK^T, softmax and PV.
-//
-// TREE: the queries are drafted tokens behind a cache (see Sm100FwdArgs), of which 128 or 256 stacked rows make a CTA.
 // =================================================================================================
 template <int D, bool DUAL>
 struct FwdSm100Smem2 {
@@ -56,10 +54,10 @@ struct FwdSm100Smem2 {
 template <int D> constexpr int kFwdPoly = D == 128 ? 1 : 2;
 enum { C_Q = 0, C_KF0, C_KF1, C_KF2, C_KE0, C_KE1, C_KE2, C_VF0, C_VF1, C_VF2, C_VE0, C_VE1, C_VE2, C_SA, C_SB, C_PA, C_PB, C_PA2, C_PB2, C_OA, C_OB, C_DRAIN, C_COUNT };
 
-template <typename T, int D, bool BIAS, bool DUAL, bool TREE>
+template <typename T, int D, bool BIAS, bool DUAL>
 __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constant__ Sm100FwdArgs a) {
-    using SM = FwdSm100Smem2<D, DUAL>;
-    constexpr int NST = SM::kStages;
+    using L = FwdSm100Smem2<D, DUAL>;
+    constexpr int NST = L::kStages;
     constexpr int NSUB = D / 64;
     constexpr int KSTEPS = D / 16;
     constexpr uint32_t TMEM_COLS = 512;
@@ -71,10 +69,10 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     extern __shared__ unsigned char smem_raw[];
     const uint32_t sbase = (smem_addr(smem_raw) + 1023u) & ~1023u;
     unsigned char* sgen = smem_raw + (sbase - smem_addr(smem_raw));
-    const uint32_t sQ = sbase + SM::oQ, sK = sbase + SM::oK, sV = sbase + SM::oV;
-    const uint32_t bars = sbase + SM::oBar;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + SM::oBar + 8 * C_COUNT);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + SM::oBar + 8 * C_COUNT + 8);
+    const uint32_t sQ = sbase + L::oQ, sK = sbase + L::oK, sV = sbase + L::oV;
+    const uint32_t bars = sbase + L::oBar;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sgen + L::oBar + 8 * C_COUNT);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sgen + L::oBar + 8 * C_COUNT + 8);
     auto bar = [&](int i) { return bars + 8u * i; };
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -103,19 +101,14 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     const int mblk = nbx / a.nsplit - 1 - bi.x / a.nsplit;
     int q_off = 0, k_off = 0, sq = a.sq, sk = a.sk;
     if (a.cu_q) { q_off = a.cu_q[b]; sq = a.cu_q[b + 1] - q_off; k_off = a.cu_k[b]; sk = a.cu_k[b + 1] - k_off; }
-    int L = 0;                                               // TREE: cached rows in front of the draft
-    if constexpr (TREE) {
-        L = tree_prefix(a.seqused_k, b, a.sk);
-        sk = (int)min((long long)L + sq, (long long)a.sk);
-    } else if (a.seqused_k) {                                // cache call: the length lives on the device
+    if (a.seqused_k) {                                       // cache call: the length lives on the device
         sk = (int)max(0LL, min((long long)a.seqused_k[b] + a.s_new, (long long)a.sk));   // an oversized entry is truncated to the capacity
     }
-    const int r0 = TREE ? mblk * (DUAL ? 128 : 256) : 0;     // TREE: first stacked row of the CTA
-    const int m0 = TREE ? 0 : mblk * (DUAL ? 1 : 2) * qpt;   // first query position of the CTA
-    if (m0 >= sq || (TREE && r0 >= sq * gq)) return;
+    const int m0 = mblk * (DUAL ? 1 : 2) * qpt;              // first query position of the CTA
+    if (m0 >= sq) return;
     if (failed) return;
     const int wl = a.wl, wr = a.causal ? 0 : a.wr;
-    const int rows_cta = min(DUAL ? 128 : 256, (sq - m0) * gq - r0);     // tile rows in use
+    const int rows_cta = min(DUAL ? 128 : 256, (sq - m0) * gq);          // tile rows in use
     const bool has_b = !DUAL && rows_cta > 128;
 
     int lo_first, hi_first, lo_last, hi_last;
@@ -123,9 +116,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     window_bounds(m0 + (rows_cta - 1) / gq, sq, sk, wl, wr, lo_last, hi_last);
     int t_lo = lo_first / 128, t_hi = hi_last < 0 ? 0 : hi_last / 128 + 1;
     if (sk <= 0 || lo_first >= sk) { t_lo = 0; t_hi = 0; }
-    if constexpr (TREE) {
-        tree_split_tiles(tree_first_any(a.tree, L), sk, a.nsplit, split, a.min_split_keys, t_lo, t_hi);
-    } else if (a.nsplit > 1) {                               // this split's share of the key tiles
+    if (a.nsplit > 1) {                                      // this split's share of the key tiles
         t_lo = max(t_lo, split * (a.keys_per_split / 128));
         t_hi = min(t_hi, (split + 1) * (a.keys_per_split / 128));
     }
@@ -133,7 +124,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     // The first 128 rows of the block may end before the last key tile of the block (under a causal mask they end one
     // tile earlier): they skip the tiles in which every one of their entries is masked.
     int nt0 = ntiles;
-    if (!TREE && has_b) {
+    if (has_b) {
         int lo_a, hi_a;
         window_bounds(m0 + qpt - 1, sq, sk, wl, wr, lo_a, hi_a);
         const int n = min(ntiles, (hi_a < 0 ? 0 : hi_a / 128 + 1) - t_lo);
@@ -142,16 +133,13 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
 
     // output row and LSE slot of tile row t (0..255) of this CTA
     auto out_row = [&](int t) -> T* {
-        t += r0;
         return reinterpret_cast<T*>(a.o) + (a.cu_q ? 0 : (int64_t)b * a.o_sb) + (int64_t)(q_off + m0 + t / gq) * a.o_ss + (int64_t)(h0 + t % gq) * a.o_sh;
     };
     auto lse_slot = [&](int t) -> float* {
-        t += r0;
         return a.lse + (a.cu_q ? 0 : (int64_t)b * a.lse_sb) + (int64_t)(h0 + t % gq) * a.lse_sh + (int64_t)(q_off + m0 + t / gq) * a.lse_ss;
     };
     // split-KV: row of tile row t in the partial buffers
     auto part_row = [&](int t) -> int64_t {
-        t += r0;
         return (int64_t)split * a.rows_all + ((int64_t)b * a.sq + m0 + t / gq) * a.hq + h0 + t % gq;
     };
 
@@ -171,9 +159,8 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
         return;
     }
 
-    const int qrow0 = TREE ? r0 : (a.cu_q ? q_off : 0) + m0;
+    const int qrow0 = (a.cu_q ? q_off : 0) + m0;
     const int qb = a.cu_q ? 0 : b;
-    const int qh = TREE ? hk : h0, qrow1 = qrow0 + (TREE ? 128 : qpt);
     // where key tile j lives: (row, outermost coordinate) of the K / V maps.  Dense and packed operands: row
     // in the batch entry; cache: row in the cache entry of this batch; paged cache: row inside the page
     // that the page table names (a tile never straddles pages when the page size is a multiple of 128; pages of
@@ -197,11 +184,11 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
         }
     };
     auto load = [&](const CUtensorMap* map, uint32_t dst, uint32_t full, int krow, int kouter, int krow2, int kouter2) {
-        mbar_expect_tx(full, SM::kKV);
+        mbar_expect_tx(full, L::kKV);
 #pragma unroll
         for (int s = 0; s < NSUB; ++s) {
-            tma_load_4d(dst + s * SM::kSub, map, full, s * 64, hk, krow, kouter);
-            if (a.kv_box == 64) tma_load_4d(dst + s * SM::kSub + 64 * 128, map, full, s * 64, hk, krow2, kouter2);
+            tma_load_4d(dst + s * L::kSub, map, full, s * 64, hk, krow, kouter);
+            if (a.kv_box == 64) tma_load_4d(dst + s * L::kSub + 64 * 128, map, full, s * 64, hk, krow2, kouter2);
         }
     };
     if (warp == 8) {
@@ -212,25 +199,19 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
             for (int i = 0; i < C_COUNT; ++i) mbar_init(bar(i), (i >= C_PA && i <= C_PB2) ? 128u : 1u);
             *abort_flag = 0;
             mbar_fence_init();
-            mbar_expect_tx(bar(C_Q), has_b ? 2 * SM::kQ : SM::kQ);
+            mbar_expect_tx(bar(C_Q), has_b ? 2 * L::kQ : L::kQ);
 #pragma unroll
-            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * SM::kSub, &a.tq, bar(C_Q), s * 64, qh, qrow0, qb);
+            for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + s * L::kSub, &a.tq, bar(C_Q), s * 64, h0, qrow0, qb);
             int krow, kouter, krow2, kouter2;
-            if constexpr (!TREE) {
-                place(0, krow, kouter, krow2, kouter2);
-                load(&a.tk, sK, bar(C_KF0), krow, kouter, krow2, kouter2);
-            }
+            place(0, krow, kouter, krow2, kouter2);
+            load(&a.tk, sK, bar(C_KF0), krow, kouter, krow2, kouter2);
             if (has_b) {
 #pragma unroll
-                for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + SM::kQ + s * SM::kSub, &a.tq, bar(C_Q), s * 64, qh, qrow1, qb);
+                for (int s = 0; s < NSUB; ++s) tma_load_4d(sQ + L::kQ + s * L::kSub, &a.tq, bar(C_Q), s * 64, h0, qrow0 + qpt, qb);
             }
-            if constexpr (!TREE) load(&a.tv, sV, bar(C_VF0), krow, kouter, krow2, kouter2);
+            load(&a.tv, sV, bar(C_VF0), krow, kouter, krow2, kouter2);
         }
         __syncwarp();
-        if constexpr (TREE) {
-            tree_load_tile<NSUB>(a, &a.tk, sK, bar(C_KF0), t_lo * 128, hk, b, lane);
-            tree_load_tile<NSUB>(a, &a.tv, sV, bar(C_VF0), t_lo * 128, hk, b, lane);
-        }
         tmem_alloc(smem_addr(tmem_slot), TMEM_COLS);
         tmem_relinquish();
     }
@@ -247,18 +228,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     static_assert(128 * 56 + 256 * 224 <= 384 * 168, "register split exceeds the CTA's allocation");
     if (warp >= 8) {
     reg_dealloc<56>();
-    if (TREE && warp == 8) {
-        bool ok = true;                                      // the whole warp, one lane a box: lanes leave together
-        for (int j = 1; j < ntiles && ok; ++j) {
-            const int st = j % NST, use = j / NST;
-            if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(C_KE0 + st), (use - 1) & 1, abort_flag, err, 1));
-            if (!ok) break;
-            tree_load_tile<NSUB>(a, &a.tk, sK + st * SM::kKV, bar(C_KF0 + st), (t_lo + j) * 128, hk, b, lane);
-            if (use > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(C_VE0 + st), (use - 1) & 1, abort_flag, err, 2));
-            if (!ok) break;
-            tree_load_tile<NSUB>(a, &a.tv, sV + st * SM::kKV, bar(C_VF0 + st), (t_lo + j) * 128, hk, b, lane);
-        }
-    } else if (warp == 8) {
+    if (warp == 8) {
         if (lane == 0) {
             bool ok = true;
             for (int j = 1; j < ntiles && ok; ++j) {
@@ -267,24 +237,24 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                 place(j, krow, kouter, krow2, kouter2);
                 if (use > 0) ok = mbar_wait(bar(C_KE0 + st), (use - 1) & 1, abort_flag, err, 1);
                 if (!ok) break;
-                load(&a.tk, sK + st * SM::kKV, bar(C_KF0 + st), krow, kouter, krow2, kouter2);
+                load(&a.tk, sK + st * L::kKV, bar(C_KF0 + st), krow, kouter, krow2, kouter2);
                 if (use > 0) ok = mbar_wait(bar(C_VE0 + st), (use - 1) & 1, abort_flag, err, 2);
                 if (!ok) break;
-                load(&a.tv, sV + st * SM::kKV, bar(C_VF0 + st), krow, kouter, krow2, kouter2);
+                load(&a.tv, sV + st * L::kKV, bar(C_VF0 + st), krow, kouter, krow2, kouter2);
             }
         }
     } else if (warp == 9) {
         {   // whole warp, one elected lane issues (see umma_ss_w)
             // descriptors of the tile origins, built once; the grouped issue adds compile-time offsets
-            const uint64_t dQ0 = umma_desc(sQ, 16, 1024), dK0 = umma_desc(sK, 16, 1024), dV0 = umma_desc(sV, SM::kSub, 1024);
+            const uint64_t dQ0 = umma_desc(sQ, 16, 1024), dK0 = umma_desc(sK, 16, 1024), dV0 = umma_desc(sV, L::kSub, 1024);
             auto issue_qk = [&](int x, int st) {
-                umma_ss_scores<KSTEPS, SM::kSub>(tmem + x * 128, umma_desc_at(dQ0, x * SM::kQ), umma_desc_at(dK0, st * SM::kKV), IDESC_QK);
+                umma_ss_scores<KSTEPS, L::kSub>(tmem + x * 128, umma_desc_at(dQ0, x * L::kQ), umma_desc_at(dK0, st * L::kKV), IDESC_QK);
                 umma_commit_w(bar(C_SA + x));
             };
             // P·V of tile x in two halves of 64 keys (16 keys = 8 columns of P, 2048 bytes of V a step): the second
             // half waits for its own barrier
             auto issue_pv = [&](int x, int st, int j) -> bool {
-                const uint64_t bv = umma_desc_at(dV0, st * SM::kKV);
+                const uint64_t bv = umma_desc_at(dV0, st * L::kKV);
                 const uint32_t d_o = tmem + 256 + x * 128, a_p = tmem + x * 128;
                 umma_ts_group4<0, 8, 0, 128>(d_o, a_p, bv, IDESC_PV, j > 0);
                 if (!mbar_wait(bar(C_PA2 + x), j & 1, abort_flag, err, 11)) return false;
@@ -296,17 +266,13 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
             if constexpr (DUAL) {
                 // stale V rows, as in the other form below
                 auto clear_stale = [&](int j, int st) {
-                    if constexpr (TREE) {
-                        tree_clear_rows<NSUB>(a, sgen + SM::oV + st * SM::kKV, (t_lo + j) * 128, L, b, lane);
-                        return;
-                    }
                     if (!a.seqused_k || (t_lo + j) * 128 + 128 <= sk) return;
                     const int first = max(0, sk - (t_lo + j) * 128);
                     const int last = a.block_table ? 128 : min(128, a.sk - (t_lo + j) * 128);
 #pragma unroll
                     for (int sub = 0; sub < NSUB; ++sub)
                         for (int idx = first * 8 + lane; idx < last * 8; idx += 32)     // 16-byte chunks of rows first .. last - 1
-                            *reinterpret_cast<uint4*>(sgen + SM::oV + st * SM::kKV + sub * SM::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(sgen + L::oV + st * L::kKV + sub * L::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
                     fence_proxy_async_smem();
                     __syncwarp();
                 };
@@ -314,7 +280,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                 auto scores = [&](int j) -> bool {
                     if (!mbar_wait(bar(C_KF0 + j % NST), (j / NST) & 1, abort_flag, err, 7)) return false;
                     tc_fence_after();
-                    umma_ss_scores<KSTEPS, SM::kSub>(tmem + (j & 1) * 128, dQ0, umma_desc_at(dK0, (j % NST) * SM::kKV), IDESC_QK);
+                    umma_ss_scores<KSTEPS, L::kSub>(tmem + (j & 1) * 128, dQ0, umma_desc_at(dK0, (j % NST) * L::kKV), IDESC_QK);
                     umma_commit_w(bar(C_SA + (j & 1)));
                     umma_commit_w(bar(C_KE0 + j % NST));
                     return true;
@@ -354,8 +320,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                 ok = mbar_wait(bar(C_VF0 + st), use & 1, abort_flag, err, 6);
                 if (ok && more) ok = mbar_wait(bar(C_KF0 + st1), use1 & 1, abort_flag, err, 7);
                 if (!ok) break;
-                if constexpr (TREE) tree_clear_rows<NSUB>(a, sgen + SM::oV + st * SM::kKV, (t_lo + j) * 128, L, b, lane);
-                else if (a.seqused_k && (t_lo + j) * 128 + 128 > sk) {
+                if (a.seqused_k && (t_lo + j) * 128 + 128 > sk) {
                     // Rows of a cache past the sequence hold whatever was there before (possibly NaN patterns): their
                     // probabilities are exact zeros, but 0 x NaN is NaN, so the V rows are cleared before the MMA.
                     // A row is 128 bytes in every 64-column sub-tile whatever the swizzle.
@@ -366,7 +331,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
 #pragma unroll
                     for (int sub = 0; sub < NSUB; ++sub)
                         for (int idx = first * 8 + lane; idx < last * 8; idx += 32)     // 16-byte chunks of rows first .. last - 1
-                            *reinterpret_cast<uint4*>(sgen + SM::oV + st * SM::kKV + sub * SM::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(sgen + L::oV + st * L::kKV + sub * L::kSub + idx * 16) = make_uint4(0, 0, 0, 0);
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
@@ -416,25 +381,12 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
         const uint32_t t_s = tmem + lane_base + x * 128;
         const uint32_t t_o = tmem + lane_base + 256 + x * 128;
         const int rows = min(128, rows_cta - x0);
-        const int qi = m0 + (r0 + x0 + r) / gq;             // query position of this thread's row
+        const int qi = m0 + (x0 + r) / gq;                  // query position of this thread's row
         int klo = 1, khi = 0;
+        if (r < rows) window_bounds(qi, sq, sk, wl, wr, klo, khi);
         int lo_l, hi_f, tmp;
-        const uint32_t* tree_row = nullptr;
-        bool there = true;                                   // TREE: the row's token exists
-        if constexpr (TREE) {
-            klo = 0x7fffffff;
-            if (r < rows) {
-                klo = tree_first_key(a.tree, b, qi, L);
-                tree_row = a.tree.bits + (int64_t)(b * a.tree.tokens + qi) * a.tree.words;
-            }
-            there = klo != 0x7fffffff;
-            lo_l = tree_first_all(a.tree, L);                // tiles inside [lo_l, hi_f] are seen by every token
-            hi_f = L - 1;
-        } else {
-            if (r < rows) window_bounds(qi, sq, sk, wl, wr, klo, khi);
-            window_bounds(m0 + x0 / gq, sq, sk, wl, wr, tmp, hi_f);
-            window_bounds(m0 + (x0 + rows - 1) / gq, sq, sk, wl, wr, lo_l, tmp);
-        }
+        window_bounds(m0 + x0 / gq, sq, sk, wl, wr, tmp, hi_f);
+        window_bounds(m0 + (x0 + rows - 1) / gq, sq, sk, wl, wr, lo_l, tmp);
         float m_used = -INFINITY, l_run = 0.f;
         // BIAS instantiation: the scores are turned into their final log2-domain values in registers (softcap, then
         // alibi, as the general kernel and the golden do), and the softmax below runs with a unit scale
@@ -482,12 +434,10 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                 if (!full) {
 #pragma unroll
                     for (int c = 2 * hh; c < 2 * hh + 2; ++c) {
-                        uint32_t vis = 0;
-                        if constexpr (TREE) vis = there ? tree_visible32(a.tree, tree_row, n0 + c * 32, klo, L) : 0u;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const int col = n0 + c * 32 + i;
-                            if (TREE ? !(vis >> i & 1) : col < klo || col > khi) sreg[c][i] = 0xff800000u;     // -inf
+                            if (col < klo || col > khi) sreg[c][i] = 0xff800000u;     // -inf
                         }
                     }
                 }
@@ -560,7 +510,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
             // All MMAs are done, so every copy has landed and been read: the exponent bases and row sums of both groups go
             // through the K buffers.
             if (ok && ntiles > 1) ok = mbar_wait(bar(C_OB), 0, abort_flag, err, 12);
-            float* merge = reinterpret_cast<float*>(sgen + SM::oK);
+            float* merge = reinterpret_cast<float*>(sgen + L::oK);
             merge[x * 256 + r] = m_used;
             merge[x * 256 + 128 + r] = l_run;
             asm volatile("barrier.cta.sync 1, 256;" ::: "memory");               // both groups, whatever became of their waits
@@ -570,7 +520,6 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
             f_b = m_b == -INFINITY ? 0.f : ex2_approx(m_b - m_used);
             l_run = merge[128 + r] * f_a + merge[384 + r] * f_b;
         }
-        if (TREE && !there) l_run = 0.f;                         // no token: whatever its q holds, zeros and no LSE
         if (ok) {
             tc_fence_after();
             const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
@@ -592,12 +541,6 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
                         tmem_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; ++i) oreg[i] = __float_as_uint(fmaf(__uint_as_float(ob[i]), f_b, __uint_as_float(oreg[i])));
-                    }
-                }
-                if constexpr (TREE) {
-                    if (!there) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) oreg[i] = 0u;
                     }
                 }
                 if (r < rows && prow) {
@@ -1152,16 +1095,15 @@ int grid_chunk(int64_t pairs, int64_t bytes_per_pair) {
     return (int)(c < 1 ? 1 : c);
 }
 
-template <typename T, int D, bool BIAS, bool DUAL, bool TREE>
+template <typename T, int D, bool BIAS, bool DUAL>
 static int launch_sm100_b(const fa_fwd_params& p, Sm100FwdArgs& a) {
     cudaStream_t st = reinterpret_cast<cudaStream_t>(p.stream);
-    auto kern = fwd_sm100_kernel2<T, D, BIAS, DUAL, TREE>;
+    auto kern = fwd_sm100_kernel2<T, D, BIAS, DUAL>;
     const int smem = FwdSm100Smem2<D, DUAL>::kBytes + 1024;
     if (int e = cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return e;
     const int qpc = 256 / a.gq;                              // query positions of a CTA
-    const int tree_rows = DUAL ? 128 : 256;
-    const unsigned nbx = (unsigned)((TREE ? (p.sq * a.gq + tree_rows - 1) / tree_rows : (p.sq + qpc - 1) / qpc) * a.nsplit);
-    a.nheads_grid = TREE || a.gq > 1 ? p.hkv : p.hq;
+    const unsigned nbx = (unsigned)(((p.sq + qpc - 1) / qpc) * a.nsplit);
+    a.nheads_grid = a.gq > 1 ? p.hkv : p.hq;
     a.chunk = grid_chunk((int64_t)p.b * a.nheads_grid, (int64_t)p.sk * p.d * 4);
     dim3 grid(a.chunk, nbx, (unsigned)(((int64_t)p.b * a.nheads_grid + a.chunk - 1) / a.chunk));
     kern<<<grid, 384, smem, st>>>(a);
@@ -1174,8 +1116,8 @@ static bool short_queries(const fa_fwd_params& p, int gq) { return (long)p.sq * 
 template <typename T, int D>
 static int launch_sm100_t(const fa_fwd_params& p, Sm100FwdArgs& a) {
     const bool bias = p.softcap > 0.f || p.alibi_slopes;
-    if (short_queries(p, a.gq)) return bias ? launch_sm100_b<T, D, true, true, false>(p, a) : launch_sm100_b<T, D, false, true, false>(p, a);
-    return bias ? launch_sm100_b<T, D, true, false, false>(p, a) : launch_sm100_b<T, D, false, false, false>(p, a);
+    if (short_queries(p, a.gq)) return bias ? launch_sm100_b<T, D, true, true>(p, a) : launch_sm100_b<T, D, false, true>(p, a);
+    return bias ? launch_sm100_b<T, D, true, false>(p, a) : launch_sm100_b<T, D, false, false>(p, a);
 }
 template <typename T, int D, bool BIAS, bool TREE>
 static int launch_sm100_wide_b(const fa_fwd_params& p, Sm100FwdArgs& a) {
@@ -1216,14 +1158,18 @@ long fwd_sm100_tree_ctas(const fa_fwd_params& p) {
     return (long)p.b * p.hkv * ((rows + tile - 1) / tile);
 }
 template <typename T>
-static int launch_tree_t(const fa_fwd_params& p, Sm100FwdArgs& a) {
-    const bool dual = p.sq * a.gq <= 128;
+static int launch_tree_wide(const fa_fwd_params& p, Sm100FwdArgs& a) {
     if (p.d == 256) return p.softcap > 0.f ? launch_sm100_wide_b<T, 256, true, true>(p, a) : launch_sm100_wide_b<T, 256, false, true>(p, a);
-    if (p.d == 192) return p.softcap > 0.f ? launch_sm100_wide_b<T, 192, true, true>(p, a) : launch_sm100_wide_b<T, 192, false, true>(p, a);
-    if (p.d == 128) return dual ? launch_sm100_b<T, 128, false, true, true>(p, a) : launch_sm100_b<T, 128, false, false, true>(p, a);
-    return dual ? launch_sm100_b<T, 64, false, true, true>(p, a) : launch_sm100_b<T, 64, false, false, true>(p, a);
+    return p.softcap > 0.f ? launch_sm100_wide_b<T, 192, true, true>(p, a) : launch_sm100_wide_b<T, 192, false, true>(p, a);
 }
-int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, float* o_part, float* lse_part) {
+// Head dims up to 128 without a cap: the kernel that shares out all key tiles evenly (tree_sm100.cu).
+// Otherwise a CTA a split, joined by the forward's combine.
+bool fwd_sm100_tree_shared(const fa_fwd_params& p) {
+    const long long tiles = ((long long)p.sk + 127) / 128 * p.b;         // at most; counted in 32 bits
+    return p.d <= 128 && !(p.softcap > 0.f) && tiles < (1ll << 30);
+}
+int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, int shares,
+                          float* o_part, float* lse_part) {
     Sm100FwdArgs a = {};
     a.gq = p.hq / p.hkv;
     a.nsplit = nsplit; a.min_split_keys = min_split_keys; a.o_part = o_part; a.lse_part = lse_part;
@@ -1243,10 +1189,17 @@ int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nspl
     a.scale_log2 = p.scale * kLog2e;
     a.softcap = p.softcap; a.cap_in = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
     a.wl = a.wr = -1;
-    const bool single = p.d <= 128 && p.softcap > 0.f;
-    note_kernel(p.d > 128 ? "sm100_tcgen05_wide" : "sm100_tcgen05_2q", single ? FORM_ONE_TILE : p.d <= 128 && p.sq * a.gq <= 128 ? FORM_SHORT_QUERIES : FORM_USUAL);
-    if (single) return launch_fwd_single_sm100(p, a, true);
-    return p.dtype == FA_F16 ? launch_tree_t<__half>(p, a) : launch_tree_t<__nv_bfloat16>(p, a);
+    a.tree_shares = shares;
+    a.min_split_tiles = min_split_keys / 128;
+    if (fwd_sm100_tree_shared(p)) {
+        const bool dual = p.sq * a.gq <= 128;
+        a.tree_blocks = dual ? 1 : (p.sq * a.gq + 255) / 256;
+        note_kernel("sm100_tcgen05_tree", dual ? FORM_SHORT_QUERIES : FORM_USUAL);
+        return launch_tree_sm100(p, a, dual);
+    }
+    note_kernel(p.d > 128 ? "sm100_tcgen05_wide" : "sm100_tcgen05_2q", p.d > 128 ? FORM_USUAL : FORM_ONE_TILE);
+    if (p.d <= 128) return launch_fwd_single_sm100(p, a, true);
+    return p.dtype == FA_F16 ? launch_tree_wide<__half>(p, a) : launch_tree_wide<__nv_bfloat16>(p, a);
 }
 
 // query group stacked into the tile rows of the two-tile kernel (dense q shorter than 128, power-of-two group)
@@ -1329,7 +1282,7 @@ static int fwd_sm100_error_flag(bool clear) {
 }
 
 int sm100_error_flag(bool clear) {
-    static int (*const flags[])(bool) = {fwd_sm100_error_flag, bwd_sm100_error_flag, bwd_wide_error_flag, fwd_single_error_flag, mla_pair_error_flag};
+    static int (*const flags[])(bool) = {fwd_sm100_error_flag, bwd_sm100_error_flag, bwd_wide_error_flag, fwd_single_error_flag, mla_pair_error_flag, tree_sm100_error_flag};
     return first_error(flags, sizeof(flags) / sizeof(flags[0]), clear);
 }
 

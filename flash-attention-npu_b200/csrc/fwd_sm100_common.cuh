@@ -40,30 +40,42 @@ struct alignas(64) Sm100FwdArgs {
     float* lse_part;                     // (nsplit, rows_all)
     int64_t rows_all;
     int chunk, nheads_grid;              // grid order, see the kernels: (batch entry, head) pairs a chunk; heads of the grid
-    // TREE instantiations: a tree of drafted tokens behind the cached rows (tree_mask.cuh).  tq covers the stacked copy of q,
-    // (dim, KV head, token x group, batch); rows of a tile are stacked rows, of which gq (any number) make a token.  Splits
-    // share out the rows that the sequence has (tree_split_tiles), min_split_keys at least.
+    // A tree of drafted tokens behind the cached rows (tree_mask.cuh).  tq covers the stacked copy of q, (dim, KV head,
+    // token x group, batch); rows of a tile are stacked rows, of which gq (any number) make a token.
+    // TREE instantiations: splits share out the rows that the sequence has (tree_split_tiles), min_split_keys at least.
     TreeMask tree;
     int min_split_keys;
+    // tree_sm100.cu: the key tiles of all sequences in one list, cut into tree_shares parts, min_split_tiles each at least
+    int tree_blocks;                     // row blocks of a KV head
+    int tree_shares, min_split_tiles;
 };
 
-// TREE: key tile at cache row `pos`, in boxes of kv_box rows (what divides a page), one lane a box.  A row past the table or
-// on a page that is not in the cache lies outside the map: zeros.  The whole warp calls it.
+// TREE: where the kv_box rows (what divides a page) from cache row `row` on live: (row, outermost coordinate) of the K / V maps.
+// A row past the table or on a page that is not in the cache lies outside the maps: zeros.
+__device__ __forceinline__ int2 tree_box(const Sm100FwdArgs& a, int row, int b) {
+    if (!a.block_table) return make_int2(row, a.cache_batch_idx ? a.cache_batch_idx[b] : b);
+    return make_int2(row % a.page_size, row < a.sk ? a.block_table[(int64_t)b * a.bt_stride + row / a.page_size] : -1);
+}
+// box number `part` of a tile
 template <int NSUB>
-__device__ __forceinline__ void tree_load_tile(const Sm100FwdArgs& a, const CUtensorMap* map, uint32_t dst, uint32_t full, int pos, int hk, int b, int lane) {
+__device__ __forceinline__ void tree_copy_box(const Sm100FwdArgs& a, const CUtensorMap* map, uint32_t dst, uint32_t full, int2 box, int part, int hk) {
+#pragma unroll
+    for (int s = 0; s < NSUB; ++s) sm100::tma_load_4d(dst + s * 128 * 128 + part * a.kv_box * 128, map, full, s * 64, hk, box.x, box.y);
+}
+// A key tile, one lane a box: `box` is the lane's, of the tile's row lane * kv_box.  The whole warp calls it.
+template <int NSUB>
+__device__ __forceinline__ void tree_copy_tile(const Sm100FwdArgs& a, const CUtensorMap* map, uint32_t dst, uint32_t full, int2 box, int hk, int lane) {
     if (lane == 0) sm100::mbar_expect_tx(full, NSUB * 128 * 128);
     __syncwarp();
-    if (lane < 128 / a.kv_box) {
-        const int row = pos + lane * a.kv_box;
-        int krow = row, kouter = a.cache_batch_idx ? a.cache_batch_idx[b] : b;
-        if (a.block_table) {
-            kouter = row < a.sk ? a.block_table[(int64_t)b * a.bt_stride + row / a.page_size] : -1;
-            krow = row % a.page_size;
-        }
-#pragma unroll
-        for (int s = 0; s < NSUB; ++s) sm100::tma_load_4d(dst + s * 128 * 128 + lane * a.kv_box * 128, map, full, s * 64, hk, krow, kouter);
-    }
+    if (lane < 128 / a.kv_box) tree_copy_box<NSUB>(a, map, dst, full, box, lane, hk);
     __syncwarp();
+}
+// ... with the lane's box looked up: the tile at cache row `pos`
+template <int NSUB>
+__device__ __forceinline__ void tree_load_tile(const Sm100FwdArgs& a, const CUtensorMap* map, uint32_t dst, uint32_t full, int pos, int hk, int b, int lane) {
+    int2 box = make_int2(0, 0);
+    if (lane < 128 / a.kv_box) box = tree_box(a, pos + lane * a.kv_box, b);
+    tree_copy_tile<NSUB>(a, map, dst, full, box, hk, lane);
 }
 // TREE: rows of the V tile at cache row n0 that no token sees may hold anything, NaN included, and 0 x NaN is NaN: rows in
 // front of every window, drafted tokens that are not there, rows behind the draft.  The whole warp calls it.
@@ -97,5 +109,8 @@ __device__ __forceinline__ void tree_clear_rows(const Sm100FwdArgs& a, unsigned 
 // capped scores, head dims up to 128: one query tile a CTA, two CTAs an SM (fwd_single_sm100.cu)
 int launch_fwd_single_sm100(const fa_fwd_params& p, Sm100FwdArgs& a, bool tree = false);
 int fwd_single_error_flag(bool clear);
+// drafted tokens, head dims 64 and 128 (tree_sm100.cu)
+int launch_tree_sm100(const fa_fwd_params& p, const Sm100FwdArgs& a, bool dual);
+int tree_sm100_error_flag(bool clear);
 
 }  // namespace fa

@@ -85,6 +85,13 @@ __device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity,
     return true;
 }
 
+// ---- programmatic dependent launch -------------------------------------------------------------------------
+// A grid launched with the attribute may start once every CTA of the grid in front has called grid_let_next_start() or left;
+// grid_wait_for_previous() waits until that grid has completed and its writes are visible.  (Without the attribute both do
+// nothing.)
+__device__ __forceinline__ void grid_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- thread-block cluster: peer shared memory and barriers -------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;

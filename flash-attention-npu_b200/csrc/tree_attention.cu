@@ -10,6 +10,7 @@
 #include "fa_utils.cuh"
 #include "fa_internal.h"
 #include "rotary_axes.cuh"
+#include "sm100_ptx.cuh"
 #include "tree_mask.cuh"
 
 namespace fa {
@@ -32,57 +33,79 @@ struct TreePrepArgs {
 };
 
 // One launch in front of the attention: ancestors of every token, the new rows into the cache (keys rotated), the queries
-// rotated and stacked.  Every CTA climbs the tree of its sequence itself (T threads, as many steps as the tree is deep):
-// at 12 levels that takes 0.3 us, less than a launch of its own.
+// rotated and stacked.  Every CTA works out the tree of its sequence itself, a thread a token, by doubling: after round k a
+// token knows its 2^k nearest ancestors, so eight rounds do for any tree of 256 tokens.  (Climbing one parent a step took 18 us
+// for a chain of 64 tokens.)
+constexpr int kPrepItems = 1;
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_constant__ TreePrepArgs a) {
-    __shared__ int s_parent[kTreeMaxTokens], s_depth[kTreeMaxTokens];
-    __shared__ unsigned char s_stored[kTreeMaxTokens];
+    // what a token has climbed to: the token there, or -1 = the cached rows, -2 = no token; and over how many
+    __shared__ short s_up[2][kTreeMaxTokens], s_depth[2][kTreeMaxTokens], s_parent[kTreeMaxTokens];
+    __shared__ uint32_t s_bits[2][kTreeMaxWords][kTreeMaxTokens];       // CTA 0: the tokens on that way
+    __shared__ uint32_t s_stored[kTreeMaxWords];
+    sm100::grid_let_next_start();
     const fa_fwd_params& p = a.p;
     const int b = blockIdx.y, tid = threadIdx.x, nt = p.sq;
     const int L = tree_prefix(p.seqused_k, b, p.sk);
     const int32_t* btab = p.block_table ? p.block_table + (int64_t)b * p.block_table_stride : nullptr;
-    if (tid < nt) s_parent[tid] = a.parents[(int64_t)b * a.parents_stride_b + tid];
-    __syncthreads();
+    const bool masks = blockIdx.x == 0;
+    int up = -2;
+    bool stored = false;
     if (tid < nt) {
         // a parent is a token in front of its child, or -1 for the last cached row; anything else: no token here, nor below it
-        int cur = tid, d = 0;
-        while (true) {
-            const int up = s_parent[cur];
-            if (up == -1) break;
-            if (up < 0 || up >= cur) { d = -1; break; }
-            cur = up;
-            ++d;
-        }
-        s_depth[tid] = d;
-        const int pos = L + tid;
-        bool stored = d >= 0 && pos < p.sk;                  // a row outside the cache is neither written nor seen
-        if (stored) stored = (uint64_t)(int64_t)(btab ? btab[pos / p.page_size] : p.cache_batch_idx ? p.cache_batch_idx[b] : b) < (uint64_t)p.kv_entries;
-        s_stored[tid] = stored;
+        const int parent = a.parents[(int64_t)b * a.parents_stride_b + tid];
+        up = parent >= -1 && parent < tid ? parent : -2;
+        const int pos = L + tid;                             // a row outside the cache is neither written nor seen
+        stored = pos < p.sk && (uint64_t)(int64_t)(btab ? btab[pos / p.page_size] : p.cache_batch_idx ? p.cache_batch_idx[b] : b) < (uint64_t)p.kv_entries;
+    }
+    s_up[0][tid] = (short)up;
+    s_parent[tid] = (short)up;
+    s_depth[0][tid] = up >= 0;
+    if (masks) {
+        for (int w = 0; w < a.words; ++w) s_bits[0][w][tid] = w == tid >> 5 ? 1u << (tid & 31) : 0u;
     }
     __syncthreads();
-    if (blockIdx.x == 0) {
+    int cur = 0;
+    for (int reach = 1; reach < nt; reach *= 2, cur ^= 1) {
+        const int to = s_up[cur][tid];
+        s_up[cur ^ 1][tid] = (short)(to >= 0 ? s_up[cur][to] : to);
+        s_depth[cur ^ 1][tid] = (short)(s_depth[cur][tid] + (to >= 0 ? s_depth[cur][to] : 0));
+        if (masks) {
+            for (int w = 0; w < a.words; ++w) s_bits[cur ^ 1][w][tid] = s_bits[cur][w][tid] | (to >= 0 ? s_bits[cur][w][to] : 0u);
+        }
+        __syncthreads();
+    }
+    const int depth = s_up[cur][tid] == -1 ? s_depth[cur][tid] : -1;
+    const uint32_t vote = __ballot_sync(0xffffffffu, stored && depth >= 0);
+    s_depth[cur ^ 1][tid] = (short)depth;                    // read below as the final depth
+    if ((tid & 31) == 0) s_stored[tid >> 5] = vote;
+    __syncthreads();
+    const short* s_final = s_depth[cur ^ 1];
+    if (masks) {
         if (tid < nt) {
-            const int d = s_depth[tid];
-            uint32_t w[kTreeMaxWords];
+            uint32_t* row = a.bits + (int64_t)(b * nt + tid) * a.words;
+            if (a.left < 0 || a.left >= depth) {
+                for (int w = 0; w < a.words; ++w) row[w] = depth >= 0 ? s_bits[cur][w][tid] & s_stored[w] : 0u;
+            } else {                                         // a window that ends inside the tree: its first left + 1 tokens
+                uint32_t seen[kTreeMaxWords];
 #pragma unroll
-            for (int i = 0; i < kTreeMaxWords; ++i) w[i] = 0;
-            for (int cur = tid, steps = 0; d >= 0 && cur >= 0 && (a.left < 0 || steps <= a.left); cur = s_parent[cur], ++steps) {
-                if (!s_stored[cur]) continue;
+                for (int i = 0; i < kTreeMaxWords; ++i) seen[i] = 0;
+                for (int at = tid, steps = 0; steps <= a.left; at = s_parent[at], ++steps) {
+#pragma unroll
+                    for (int i = 0; i < kTreeMaxWords; ++i)
+                        if (i == at >> 5) seen[i] |= 1u << (at & 31);
+                }
 #pragma unroll
                 for (int i = 0; i < kTreeMaxWords; ++i)
-                    if (i == cur >> 5) w[i] |= 1u << (cur & 31);
+                    if (i < a.words) row[i] = seen[i] & s_stored[i];
             }
-            uint32_t* row = a.bits + (int64_t)(b * nt + tid) * a.words;
-#pragma unroll
-            for (int i = 0; i < kTreeMaxWords; ++i)
-                if (i < a.words) row[i] = w[i];
-            a.depth[b * nt + tid] = d;
+            a.depth[b * nt + tid] = depth;
         }
-        const uint32_t vote = __ballot_sync(0xffffffffu, tid < nt && s_stored[tid]);
         if ((tid & 31) == 0 && (tid >> 5) < a.words) a.keys[b * a.words + (tid >> 5)] = vote;
     }
-    const int item = blockIdx.x * kTreeMaxTokens + tid;
+#pragma unroll 2
+    for (int k = 0; k < kPrepItems; ++k) {
+    const int item = (blockIdx.x * kPrepItems + k) * kTreeMaxTokens + tid;
     if (item >= a.items) return;
     const bool is_q = item >= a.items_kv, is_v = !is_q && item >= a.items_k;
     const int at = is_q ? item - a.items_kv : is_v ? item - a.items_k : item;
@@ -95,7 +118,7 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
         src = reinterpret_cast<const T*>(p.q.ptr) + (int64_t)b * p.q.stride_b + (int64_t)t * p.q.stride_s + (int64_t)h * p.q.stride_h;
         dst = reinterpret_cast<T*>(a.q_stack) + (((int64_t)b * p.hkv + hk) * nt * a.g + (int64_t)t * a.g + h % a.g) * p.d;
     } else {
-        if (!s_stored[t]) return;
+        if (!(s_stored[t >> 5] >> (t & 31) & 1)) continue;
         const int pos = L + t;
         int64_t outer, rin;
         if (btab) {
@@ -112,7 +135,7 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
     }
     const int rd = is_v ? 0 : a.ro.rd;
     RotaryRows rows = {};
-    if (rd) rows = a.ro.positions ? rotary_rows(a.ro, b, t) : same_row(a.ro, L + max(s_depth[t], 0));
+    if (rd) rows = a.ro.positions ? rotary_rows(a.ro, b, t) : same_row(a.ro, L + max((int)s_final[t], 0));
     if constexpr (VEC) {
         const uint4* s4 = reinterpret_cast<const uint4*>(src);
         uint4* d4 = reinterpret_cast<uint4*>(dst);
@@ -133,21 +156,40 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
     } else {
         for (int e = u * 16; e < min(n, u * 16 + 16); ++e) dst[e] = rd ? turn_elem<T, T>(src, e, a.ro, rows, 1.f) : src[e];
     }
+    }
 }
 
 struct TreePlan {
-    int nsplit, min_keys, words, sm100;
+    int nsplit, min_keys, words, sm100, shared, shares;
     size_t bits, depth, keys, q, o, lse, total;
 };
 
-// Splits of the keys.  min_keys: what a split has at least; more splits than that leave none to the short sequences, whose CTAs
-// then only write that they are empty.
+// tree_sm100.cu: lanes (row blocks of KV heads), and into how many shares the list of key tiles is cut.  All CTAs do about the
+// same, so what counts is how many of them an SM gets one after the other: the fewest such rounds a share, one round if that
+// leaves no more than a twelfth of the SMs without work.
+long lanes_of(const fa_fwd_params& p) {
+    const long rows = (long)p.sq * (p.hq / p.hkv);
+    return p.hkv * (rows <= 128 ? 1 : (rows + 255) / 256);
+}
+int shares_of(const fa_fwd_params& p) {
+    const long lanes = lanes_of(p), sms = sm_count();
+    long best = 1;
+    double best_cost = 0;
+    for (long n = 1; n <= 8 * sms && (n == 1 || n * lanes <= 3 * sms); ++n) {
+        const double rounds = (double)((n * lanes + sms - 1) / sms), cost = rounds / n + 0.08 * rounds * lanes / sms;
+        if (n == 1 || cost < best_cost) { best = n; best_cost = cost; }
+    }
+    return (int)best;
+}
+
+// Splits of the keys.  min_keys: what a split, or a CTA's share of the key tiles, has at least.
 void plan_tree(const fa_fwd_params& p, TreePlan& plan) {
     plan = {};
     const long rows = (long)p.sq * (p.hq / p.hkv);
     plan.words = (p.sq + 31) / 32;
-    plan.min_keys = 512;
     plan.sm100 = fwd_sm100_tree_supported(p) ? 1 : 0;
+    plan.shared = plan.sm100 && fwd_sm100_tree_shared(p);
+    plan.min_keys = plan.shared ? 256 : 512;
     const long base = plan.sm100 ? fwd_sm100_tree_ctas(p) : (long)p.b * p.hkv * ((rows + kGenericBM - 1) / kGenericBM);
     const long most = ((long)p.sk + plan.min_keys - 1) / plan.min_keys;
     const long waves = plan.sm100 ? 2 : 4;
@@ -162,6 +204,15 @@ void plan_tree(const fa_fwd_params& p, TreePlan& plan) {
     plan.keys = plan.depth + align256(toks * 4);
     plan.q = plan.keys + align256((size_t)p.b * plan.words * 4);
     plan.o = plan.q + align256(toks * p.hq * p.d * 2);
+    if (plan.shared) {                                       // at most two pieces a CTA
+        plan.shares = shares_of(p);
+        // a call that asks for n splits gets shares of at least that part of the longest sequence
+        if (p.num_splits > 0) plan.min_keys = (int)((((long)p.sk + 127) / 128 + p.num_splits - 1) / p.num_splits) * 128;
+        const size_t pieces = plan.shares == 1 ? 0 : (size_t)lanes_of(p) * plan.shares * 2 * (rows <= 128 ? 128 : 256);
+        plan.lse = plan.o + align256(pieces * p.d * 4);
+        plan.total = plan.lse + align256(pieces * 4);
+        return;
+    }
     plan.lse = plan.o + (plan.nsplit > 1 ? align256((size_t)plan.nsplit * toks * p.hq * p.d * 4) : 0);
     plan.total = plan.lse + (plan.nsplit > 1 ? align256((size_t)plan.nsplit * toks * p.hq * 4) : 0);
 }
@@ -255,7 +306,7 @@ int run_tree(const fa_tree_params& t) {
     a.items_k = p.k_new.ptr ? p.sq * p.hkv * a.uk : 0;
     a.items_kv = a.items_k + (p.k_new.ptr ? p.sq * p.hkv * a.uv : 0);
     a.items = a.items_kv + p.sq * p.hq * a.uk;
-    const dim3 grid((a.items + kTreeMaxTokens - 1) / kTreeMaxTokens, p.b);
+    const dim3 grid((a.items + kPrepItems * kTreeMaxTokens - 1) / (kPrepItems * kTreeMaxTokens), p.b);
     const bool vec = tree_vec_ok(p);
     if (p.dtype == FA_F16) {
         if (vec) tree_prep_kernel<__half, true><<<grid, kTreeMaxTokens, 0, st>>>(a);
@@ -273,9 +324,10 @@ int run_tree(const fa_tree_params& t) {
     p.q.stride_s = p.d;
     p.q.stride_h = rows * p.d;
     p.q.stride_b = p.hkv * rows * p.d;
-    float* o_part = plan.nsplit > 1 ? reinterpret_cast<float*>(ws + plan.o) : nullptr;
-    float* lse_part = plan.nsplit > 1 ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;
-    const int e = plan.sm100 ? launch_fwd_sm100_tree(p, mask, plan.nsplit, plan.min_keys, o_part, lse_part)
+    float* o_part = plan.shared || plan.nsplit > 1 ? reinterpret_cast<float*>(ws + plan.o) : nullptr;
+    float* lse_part = plan.shared || plan.nsplit > 1 ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;
+    if (plan.shared) return launch_fwd_sm100_tree(p, mask, 1, plan.min_keys, plan.shares, o_part, lse_part);
+    const int e = plan.sm100 ? launch_fwd_sm100_tree(p, mask, plan.nsplit, plan.min_keys, 1, o_part, lse_part)
                              : launch_fwd_generic_tree(p, mask, plan.nsplit, plan.min_keys, o_part, lse_part);
     if (e) return e;
     return plan.nsplit > 1 ? launch_fwd_combine(p, plan.nsplit, o_part, lse_part, 0) : FA_OK;

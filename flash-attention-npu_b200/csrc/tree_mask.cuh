@@ -20,16 +20,25 @@ struct TreeMask {
     int left;                    // window to the left, -1 = none
 };
 
+// Entries of a CTA's share of a list of `total` key tiles
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline int tree_share(int total, int ctas, int at_least) {
+    const int even = total / ctas + (total % ctas != 0);
+    return even > at_least ? even : at_least;
+}
+
 #ifdef __CUDACC__
 // Length of the cached prefix: a stale or oversized entry is truncated to the capacity, as in the other cache calls.
 __device__ __forceinline__ int tree_prefix(const int32_t* seqused, int b, int capacity) { return max(0, min(seqused[b], capacity)); }
 
 // First cached row that token t of sequence b sees (the prefix ends at L): past every row where there is no token.
-__device__ __forceinline__ int tree_first_key(const TreeMask& m, int b, int t, int L) {
-    const int depth = m.depth[b * m.tokens + t];
+__device__ __forceinline__ int tree_first_key(const TreeMask& m, int depth, int L) {
     if (depth < 0) return 0x7fffffff;
     return m.left < 0 ? 0 : (int)max(0ll, (long long)L + depth - m.left);
 }
+__device__ __forceinline__ int tree_first_key(const TreeMask& m, int b, int t, int L) { return tree_first_key(m, m.depth[b * m.tokens + t], L); }
 // ... that any token can see, and the first one that every token sees
 __device__ __forceinline__ int tree_first_any(const TreeMask& m, int L) { return m.left < 0 ? 0 : (int)max(0ll, (long long)L - m.left); }
 __device__ __forceinline__ int tree_first_all(const TreeMask& m, int L) { return m.left < 0 ? 0 : (int)max(0ll, (long long)L + m.tokens - 1 - m.left); }
@@ -51,6 +60,11 @@ __device__ __forceinline__ uint32_t tree_visible32(const TreeMask& m, const uint
     uint32_t v = first >= L ? 0u : bit_range(first > base ? min(first - base, 32) : 0, L - base);
     if (base + 32 > L && base < L + m.tokens) v |= tree_bits32(row, m.words, base - L);
     return v;
+}
+// Key tiles of a sequence: `n` from tile `lo` on
+__device__ __forceinline__ void tree_tiles(const TreeMask& m, int L, int sk, int& lo, int& n) {
+    lo = tree_first_any(m, L) / 128;
+    n = max(0, (sk + 127) / 128 - lo);
 }
 // Keys of one split: the rows that any token can see, shared out evenly in whole 128-key tiles, at least min_keys a split
 // (the lengths are on the device, so every CTA works this out for its own sequence).  -> [t_lo, t_hi) in tiles

@@ -292,9 +292,9 @@ def test_depths_of_the_reference():
 
 
 @pytest.mark.parametrize("d,softcap,page,hq,t,name,form", [
-    (128, 0.0, 64, 8, 16, "sm100_tcgen05_2q", 1), (64, 0.0, 16, 14, 40, "sm100_tcgen05_2q", 0), (128, 20.0, 0, 6, 9, "sm100_tcgen05_2q", 2),
+    (128, 0.0, 64, 8, 16, "sm100_tcgen05_tree", 1), (64, 0.0, 16, 14, 40, "sm100_tcgen05_tree", 0), (128, 20.0, 0, 6, 9, "sm100_tcgen05_2q", 2),
     (256, 0.0, 32, 4, 9, "sm100_tcgen05_wide", 0), (192, 5.0, 128, 4, 9, "sm100_tcgen05_wide", 0), (96, 0.0, 64, 4, 9, "generic_mma", 0),
-    (128, 0.0, 48, 8, 16, "sm100_tcgen05_2q", 1), (128, 0.0, 40, 8, 16, "generic_mma", 0)])
+    (128, 0.0, 48, 8, 16, "sm100_tcgen05_tree", 1), (128, 0.0, 40, 8, 16, "generic_mma", 0)])
 def test_which_kernel_runs(d, softcap, page, hq, t, name, form):
     check(make(torch.bfloat16, d, hq, 2, [150, 300], t, page, seed=d + page), softcap=softcap)
     assert capi.last_kernel() == name and capi.lib.fa_debug_get(8) == form
@@ -309,3 +309,22 @@ def test_the_general_kernels_agree():
     finally:
         capi.lib.fa_set_kernel_policy(0)
     check(c)
+
+
+@pytest.mark.parametrize("hq,hkv,t,lens", [
+    (8, 2, 16, [900, 5, 0, 130, 2000, 64, 300]),          # shares that end inside sequences, sequences inside a share
+    (8, 8, 33, [1] * 40),                                 # more units than CTAs, a tile each
+    (32, 1, 20, [3000, 1, 1, 1]),                         # several row blocks of a KV head
+    (4, 1, 200, [700, 90]),
+    (2, 2, 3, [12000]),                                   # one sequence over many CTAs
+    (16, 16, 2, [40, 700] * 20),                          # 640 units
+])
+@pytest.mark.parametrize("left", [-1, 100])
+def test_shares_of_the_key_tiles(hq, hkv, t, lens, left):
+    check(make(torch.bfloat16, 64, hq, hkv, lens, t, 64, seed=t + len(lens)), left=left)
+    assert capi.last_kernel() == "sm100_tcgen05_tree"
+
+
+def test_many_sequences():
+    """More sequences than one step of the search for a CTA's first one looks at."""
+    check(make(torch.bfloat16, 64, 2, 1, [(37 * i) % 300 for i in range(1100)], 2, 64, seed=3))
