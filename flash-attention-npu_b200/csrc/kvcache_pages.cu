@@ -18,6 +18,7 @@ namespace {
 constexpr int kChunk = 4096;                 // pages whose free ones are listed together
 constexpr int kMaxPages = 1 << 24;
 constexpr int kMaxViews = 56;                // caches (or stacks of them) of one launch: they travel as kernel parameters
+constexpr int kSmallThreads = 1024;         // of the one block that does a small call
 constexpr int kPiece = 32768;                // bytes of a page that a CTA copies at a time
 
 __device__ __forceinline__ int pages_of(long long rows, int page_size, int width) {
@@ -41,6 +42,7 @@ struct PoolArgs {
     // workspace
     int32_t* need;               // (rows): entries to fill; fork: 1 = the row gets a copy of its partly filled page
     int32_t* first;              // (rows): reserve: first entry to fill; fork: its partly filled page, -1 = none
+    int32_t* fill;               // (rows): fork: its length
     int32_t* free_count;         // (chunks)
     int32_t* free_list;          // (pages): the free pages of chunk c from entry c * kChunk on, ascending
     int32_t* missing;
@@ -51,14 +53,17 @@ struct PoolArgs {
     int32_t* new_seqlens;        // (n)
 };
 
-// ---- free pages, chunk by chunk: 256 threads, 16 consecutive pages each -------------------------------------------------
+// ---- free pages, chunk by chunk: THREADS threads, kChunk / THREADS consecutive pages each ---------------------------------
+template <int THREADS>
 __device__ void list_free(const PoolArgs& a, int chunk) {
-    __shared__ int s_warp[8];
+    constexpr int EACH = kChunk / THREADS, WARPS = THREADS / 32;
+    __shared__ int s_warp[WARPS];
+    __syncthreads();                                         // may be called again for the next chunk
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int p0 = chunk * kChunk + tid * 16;
+    const int p0 = chunk * kChunk + tid * EACH;
     uint32_t zero = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) zero |= (uint32_t)(p0 + i < a.num_pages && a.refs[min(p0 + i, a.num_pages - 1)] == 0) << i;
+    for (int i = 0; i < EACH; ++i) zero |= (uint32_t)(p0 + i < a.num_pages && a.refs[min(p0 + i, a.num_pages - 1)] == 0) << i;
     const int mine = __popc(zero);
     int upto = mine;
 #pragma unroll
@@ -70,7 +75,7 @@ __device__ void list_free(const PoolArgs& a, int chunk) {
     __syncthreads();
     int before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
         before += w < warp ? s_warp[w] : 0;
         total += s_warp[w];
     }
@@ -110,12 +115,8 @@ __device__ int free_page(const PoolArgs& a, int chunks, long long slot) {
 }
 
 // ---- reserve ----------------------------------------------------------------------------------------------------------
-// Launch 1: the first row_blocks blocks count what each row needs (a warp a row), the others list free pages.
-__global__ void __launch_bounds__(256) reserve_count_kernel(const __grid_constant__ PoolArgs a, int row_blocks) {
-    if ((int)blockIdx.x >= row_blocks) { list_free(a, blockIdx.x - row_blocks); return; }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.missing = 0;
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= a.b) return;
+// what a row needs; a warp a row
+__device__ void reserve_count(const PoolArgs& a, int row, int lane) {
     const int n = pages_of((long long)a.seqlens[row] + a.extra, a.page_size, a.width);
     const int32_t* t = a.table + row * a.table_stride;
     int need = 0, first = n;
@@ -129,12 +130,8 @@ __global__ void __launch_bounds__(256) reserve_count_kernel(const __grid_constan
     }
     if (lane == 0) { a.need[row] = need; a.first[row] = first; }
 }
-// Launch 2: every row takes the pages behind those of the rows in front of it.
-__global__ void __launch_bounds__(256) reserve_take_kernel(const __grid_constant__ PoolArgs a, int chunks) {
-    const int row0 = blockIdx.x * 8, row = row0 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    long long slot = block_sum(a.need, row0);
-    if (row >= a.b) return;
-    for (int r = row0; r < row; ++r) slot += a.need[r];
+// takes the free pages from number `slot` on
+__device__ void reserve_take(const PoolArgs& a, int row, int lane, int chunks, long long slot) {
     const int need = a.need[row];
     if (need == 0) return;
     const int n = pages_of((long long)a.seqlens[row] + a.extra, a.page_size, a.width);
@@ -155,6 +152,34 @@ __global__ void __launch_bounds__(256) reserve_take_kernel(const __grid_constant
     for (int d = 16; d > 0; d >>= 1) lacking += __shfl_xor_sync(0xffffffffu, lacking, d);
     if (lane == 0 && lacking) atomicAdd(a.missing, lacking);
 }
+// Launch 1: the first row_blocks blocks count, the others list free pages.
+__global__ void __launch_bounds__(256) reserve_count_kernel(const __grid_constant__ PoolArgs a, int row_blocks) {
+    if ((int)blockIdx.x >= row_blocks) { list_free<256>(a, blockIdx.x - row_blocks); return; }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.missing = 0;
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row < a.b) reserve_count(a, row, threadIdx.x & 31);
+}
+// Launch 2: every row takes the pages behind those of the rows in front of it.
+__global__ void __launch_bounds__(256) reserve_take_kernel(const __grid_constant__ PoolArgs a, int chunks) {
+    const int row0 = blockIdx.x * 8, row = row0 + (threadIdx.x >> 5);
+    long long slot = block_sum(a.need, row0);
+    if (row >= a.b) return;
+    for (int r = row0; r < row; ++r) slot += a.need[r];
+    reserve_take(a, row, threadIdx.x & 31, chunks, slot);
+}
+// Few rows and pages: one block does both, which saves a launch.
+__global__ void __launch_bounds__(kSmallThreads) reserve_small_kernel(const __grid_constant__ PoolArgs a, int chunks) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) *a.missing = 0;
+    for (int row = warp; row < a.b; row += kSmallThreads / 32) reserve_count(a, row, lane);
+    for (int c = 0; c < chunks; ++c) list_free<kSmallThreads>(a, c);
+    __syncthreads();
+    long long slot = 0;
+    for (int row = 0, r = warp; r < a.b; r += kSmallThreads / 32) {
+        for (; row < r; ++row) slot += a.need[row];
+        reserve_take(a, r, lane, chunks, slot);
+    }
+}
 
 // ---- free -------------------------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256) free_kernel(const __grid_constant__ PoolArgs a) {
@@ -170,10 +195,8 @@ __global__ void __launch_bounds__(256) free_kernel(const __grid_constant__ PoolA
 }
 
 // ---- fork -------------------------------------------------------------------------------------------------------------
-// Launch 1 (a warp a row): children share their parent's pages; with the parents replaced, the old rows let go of theirs.
-__global__ void __launch_bounds__(256) fork_share_kernel(const __grid_constant__ PoolArgs a) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.missing = 0;
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+// A warp a row: children share their parent's pages; with the parents replaced, the old rows (n ..) let go of theirs.
+__device__ void fork_share(const PoolArgs& a, int row, int lane) {
     if (row < a.n) {
         const int parent = a.parents[row];
         const bool valid = parent >= 0 && parent < a.b;
@@ -191,19 +214,16 @@ __global__ void __launch_bounds__(256) fork_share_kernel(const __grid_constant__
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, d));
-        if (lane == 0) { a.first[row] = last; a.new_seqlens[row] = len; }
+        if (lane == 0) { a.first[row] = last; a.fill[row] = len; a.new_seqlens[row] = len; }
     } else if (!a.keep_parents && row - a.n < a.b) {
         const int32_t* t = a.table + (row - a.n) * a.table_stride;
         for (int j = lane; j < a.width; j += 32)
             if (t[j] >= 0 && in_pool(t[j], a.num_pages)) drop_ref(a.refs, t[j]);
     }
 }
-// Launch 2: which rows need a page of their own.  Of the c rows that hold the same partly filled page, with e holders
+// Which rows need a page of their own.  Of the c rows that hold the same partly filled page, with e holders
 // elsewhere (count = c + e), row number i of them takes a copy when i < c + e - 1: all but the last, or all where e > 0.
-__global__ void __launch_bounds__(256) fork_count_kernel(const __grid_constant__ PoolArgs a, int row_blocks) {
-    if ((int)blockIdx.x >= row_blocks) { list_free(a, blockIdx.x - row_blocks); return; }
-    const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (row >= a.n) return;
+__device__ void fork_count(const PoolArgs& a, int row, int lane) {
     const int page = a.first[row];
     int before = 0;
     if (page >= 0) {
@@ -213,6 +233,24 @@ __global__ void __launch_bounds__(256) fork_count_kernel(const __grid_constant__
         for (int d = 16; d > 0; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
     }
     if (lane == 0) a.need[row] = page >= 0 && a.refs[page] - before > 1;
+}
+__global__ void __launch_bounds__(256) fork_share_kernel(const __grid_constant__ PoolArgs a) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.missing = 0;
+    fork_share(a, blockIdx.x * 8 + (threadIdx.x >> 5), threadIdx.x & 31);
+}
+__global__ void __launch_bounds__(256) fork_count_kernel(const __grid_constant__ PoolArgs a, int row_blocks) {
+    if ((int)blockIdx.x >= row_blocks) { list_free<256>(a, blockIdx.x - row_blocks); return; }
+    const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row < a.n) fork_count(a, row, threadIdx.x & 31);
+}
+// Few rows and pages: one block does both.
+__global__ void __launch_bounds__(kSmallThreads) fork_small_kernel(const __grid_constant__ PoolArgs a, int chunks) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) *a.missing = 0;
+    for (int row = warp; row < a.n + (a.keep_parents ? 0 : a.b); row += kSmallThreads / 32) fork_share(a, row, lane);
+    __syncthreads();
+    for (int row = warp; row < a.n; row += kSmallThreads / 32) fork_count(a, row, lane);
+    for (int c = 0; c < chunks; ++c) list_free<kSmallThreads>(a, c);
 }
 
 // ---- copies -----------------------------------------------------------------------------------------------------------
@@ -239,7 +277,7 @@ __device__ __forceinline__ void copy_piece(const View& v, const char* src, char*
         const int64_t r = o / row_bytes, rest = o % row_bytes;
         return r * v.row + rest / v.seg * v.head + rest % v.seg;
     };
-    constexpr int N = 8;
+    constexpr int N = 4;
     for (int64_t o = from + (int64_t)threadIdx.x * sizeof(V); o < to; o += (int64_t)N * 256 * sizeof(V)) {
         V x[N];
         int64_t where[N];
@@ -255,7 +293,7 @@ __device__ __forceinline__ void copy_piece(const View& v, const char* src, char*
     }
 }
 
-__global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyArgs a) {
+__global__ void __launch_bounds__(256, 4) copy_kernel(const __grid_constant__ CopyArgs a) {
     const int row = blockIdx.x / a.per_row, part = blockIdx.x % a.per_row;
     int src, dst, rows = a.page_size;
     if (a.src) {
@@ -264,11 +302,10 @@ __global__ void __launch_bounds__(256) copy_kernel(const __grid_constant__ CopyA
         if (!in_pool(src, a.num_pages) || !in_pool(dst, a.num_pages) || src == dst) return;
     } else {
         const PoolArgs& p = a.pool;
-        if (!p.need[row]) return;
+        const int need = p.need[row], len = p.fill[row];
         src = p.first[row];
+        if (!need) return;
         dst = free_page(p, a.chunks, block_sum(p.need, row));
-        const int parent = p.parents[row];
-        const int len = (int)max(0ll, min((long long)p.seqlens[parent], (long long)p.width * p.page_size));
         rows = len % a.page_size;
         if (a.first_launch && part == 0 && threadIdx.x == 0) {
             p.new_table[(int64_t)row * p.width + len / a.page_size] = dst;
@@ -394,12 +431,16 @@ __global__ void __launch_bounds__(128) compact_kernel(const __grid_constant__ Co
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 int chunks_of(const fa_pages_params& p) { return (p.num_pages + kChunk - 1) / kChunk; }
 
+// One block instead of two launches of several: up to 64 rows, 1024 table entries a warp and two lists of pages.
+bool small_pool(const fa_pages_params& p, int rows) { return rows <= 64 && (int64_t)(rows + 31) / 32 * p.width <= 1024 && chunks_of(p) <= 2; }
+
 size_t workspace(const fa_pages_params& p, int rows, PoolArgs* a) {
-    const size_t need = 0, first = align256((size_t)rows * 4), count = 2 * first, list = count + align256((size_t)chunks_of(p) * 4);
+    const size_t need = 0, first = align256((size_t)rows * 4), fill = 2 * first, count = 3 * first, list = count + align256((size_t)chunks_of(p) * 4);
     if (a) {
         char* ws = reinterpret_cast<char*>(p.workspace);
         a->need = reinterpret_cast<int32_t*>(ws + need);
         a->first = reinterpret_cast<int32_t*>(ws + first);
+        a->fill = reinterpret_cast<int32_t*>(ws + fill);
         a->free_count = reinterpret_cast<int32_t*>(ws + count);
         a->free_list = reinterpret_cast<int32_t*>(ws + list);
     }
@@ -470,8 +511,8 @@ int launch_copies(const fa_pages_params& p, const PoolArgs& pool, bool lists, cu
             a.views[i] = view_of(p.caches[v0 + i]);
             units += (int64_t)a.views[i].caches * (((int64_t)p.page_size * a.views[i].heads * a.views[i].seg + kPiece - 1) / kPiece);
         }
-        // CTAs of a row: one a unit, but no more than about 16 an SM over all rows
-        int64_t per = (16ll * sm_count() + p.n - 1) / p.n;
+        // CTAs of a row: one a unit, but no more than what four to an SM make, so that each works out its page once
+        int64_t per = (4ll * sm_count() + p.n - 1) / p.n;
         if (per > units) per = units;
         a.per_row = (int)(per < 1 ? 1 : per);
         copy_kernel<<<(unsigned)(a.per_row * p.n), 256, 0, st>>>(a);
@@ -491,6 +532,11 @@ int run_reserve(const fa_pages_params& p) {
     workspace(p, p.b, &a);
     const int rows = (p.b + 7) / 8 > 0 ? (p.b + 7) / 8 : 1, chunks = chunks_of(p);
     mark_kernel(st);
+    if (small_pool(p, p.b)) {
+        reserve_small_kernel<<<1, kSmallThreads, 0, st>>>(a, chunks);
+        mark_kernel(st);
+        return cuda_ok(cudaGetLastError(), "reserve launch");
+    }
     reserve_count_kernel<<<rows + chunks, 256, 0, st>>>(a, rows);
     mark_kernel(st);
     if (int e = cuda_ok(cudaGetLastError(), "reserve launch")) return e;
@@ -524,6 +570,12 @@ int run_fork(const fa_pages_params& p) {
     workspace(p, p.n, &a);
     const int share = p.n + (p.keep_parents ? 0 : p.b);
     mark_kernel(st);
+    if (small_pool(p, share)) {
+        fork_small_kernel<<<1, kSmallThreads, 0, st>>>(a, chunks_of(p));
+        mark_kernel(st);
+        if (int e = cuda_ok(cudaGetLastError(), "fork launch")) return e;
+        return p.n ? launch_copies(p, a, false, st) : FA_OK;
+    }
     fork_share_kernel<<<(share + 7) / 8 > 0 ? (share + 7) / 8 : 1, 256, 0, st>>>(a);
     mark_kernel(st);
     if (int e = cuda_ok(cudaGetLastError(), "fork launch")) return e;

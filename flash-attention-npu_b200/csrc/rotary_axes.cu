@@ -4,7 +4,8 @@
 //
 // Bound by HBM: (Hq + Hkv) D elements a token are read and written once, 4 bytes each way together.  One launch does q and k,
 // so that the tables and positions are looked up once a token: a thread keeps the eight cosines and sines of its unit (two
-// 16-byte chunks that hold each other's partners) in registers and walks over heads.
+// 16-byte chunks that hold each other's partners) in registers and walks over heads.  16384 tokens of 32 + 8 heads of 128, bf16,
+// q and k slices of one projection: 59.7 us a direction, 86 % of the copy rate; 57.5 with one axis, 6.3 for 512 tokens, 4.3 for 33.
 #include <cstring>
 #include "fa_utils.cuh"
 #include "fa_internal.h"
@@ -24,7 +25,8 @@ struct RotaryArgs {
     float sign;                      // -1: turn back
 };
 
-constexpr int kThreads = 128;
+// 64 threads: 59.7 us for the above; 128: 59.8, 256: 73
+constexpr int kThreads = 64;
 
 // thread -> (unit, head lane) of a token; blockIdx.x: token x group of heads
 template <typename T, typename TT, bool VEC>
@@ -60,7 +62,9 @@ __global__ void __launch_bounds__(kThreads) rotary_axes_kernel(const __grid_cons
         dst = reinterpret_cast<T*>(y.ptr) + (int64_t)b * y.stride_b + (int64_t)t * y.stride_s + (int64_t)hh * y.stride_h;
     };
     if constexpr (VEC) {
-        constexpr int N = 4;                                 // heads in flight
+        // heads in flight: 2, read and written past the caches' usual policy (nothing comes back for them): 59.7 us for the above;
+        // without that 61.4, with 1 / 4 / 5 heads 65.6 / 65.8 / 69
+        constexpr int N = 2;
         for (int i = 0; i < a.iters; i += N) {
             uint4 xa[N], xb[N];
             T* out[N];
@@ -71,8 +75,8 @@ __global__ void __launch_bounds__(kThreads) rotary_axes_kernel(const __grid_cons
                 if (i + k < a.iters && h < heads) {
                     const T* src;
                     row_of(h, src, out[k]);
-                    xa[k] = reinterpret_cast<const uint4*>(src)[lo];
-                    if (two) xb[k] = reinterpret_cast<const uint4*>(src)[hi];
+                    xa[k] = __ldcs(reinterpret_cast<const uint4*>(src) + lo);
+                    if (two) xb[k] = __ldcs(reinterpret_cast<const uint4*>(src) + hi);
                 }
             }
 #pragma unroll
@@ -80,8 +84,8 @@ __global__ void __launch_bounds__(kThreads) rotary_axes_kernel(const __grid_cons
                 if (!out[k]) continue;
                 uint4 ya = xa[k], yb = xb[k];
                 if (turned) turn8<T>(xa[k], xb[k], c, s, a.ro.interleaved, ya, yb);
-                reinterpret_cast<uint4*>(out[k])[lo] = ya;
-                if (two) reinterpret_cast<uint4*>(out[k])[hi] = yb;
+                __stcs(reinterpret_cast<uint4*>(out[k]) + lo, ya);
+                if (two) __stcs(reinterpret_cast<uint4*>(out[k]) + hi, yb);
             }
         }
     } else {
