@@ -1147,8 +1147,8 @@ static int tree_box(const fa_fwd_params& p) {
 }
 bool fwd_sm100_tree_supported(const fa_fwd_params& p) {
     if (kernel_policy() != 0) return false;
-    if (p.d != 64 && p.d != 128 && p.d != 192 && p.d != 256) return false;
-    if (tree_box(p) < 16 || p.kv_entries > (1 << 24) || !(p.scale > 0.f) || p.sk <= 0) return false;
+    if (p.d % 8 || p.d > 256) return false;                  // the kernels run the next of 64 / 128 / 192 / 256, as in the forward
+    if (tree_box(p) < 8 || p.kv_entries > (1 << 24) || !(p.scale > 0.f) || p.sk <= 0) return false;
     for (const fa_tensor* t : {&p.k, &p.v})
         if (t->stride_h <= 0 || t->stride_s <= 0 || t->stride_b <= 0) return false;
     return encode_fn() != nullptr;
@@ -1159,7 +1159,7 @@ long fwd_sm100_tree_ctas(const fa_fwd_params& p) {
 }
 template <typename T>
 static int launch_tree_wide(const fa_fwd_params& p, Sm100FwdArgs& a) {
-    if (p.d == 256) return p.softcap > 0.f ? launch_sm100_wide_b<T, 256, true, true>(p, a) : launch_sm100_wide_b<T, 256, false, true>(p, a);
+    if (p.d > 192) return p.softcap > 0.f ? launch_sm100_wide_b<T, 256, true, true>(p, a) : launch_sm100_wide_b<T, 256, false, true>(p, a);
     return p.softcap > 0.f ? launch_sm100_wide_b<T, 192, true, true>(p, a) : launch_sm100_wide_b<T, 192, false, true>(p, a);
 }
 // Head dims up to 128 without a cap: the kernel that shares out all key tiles evenly (tree_sm100.cu).

@@ -109,7 +109,7 @@ __device__ __forceinline__ void tree_clear_rows(const Sm100FwdArgs& a, unsigned 
 // capped scores, head dims up to 128: one query tile a CTA, two CTAs an SM (fwd_single_sm100.cu)
 int launch_fwd_single_sm100(const fa_fwd_params& p, Sm100FwdArgs& a, bool tree = false);
 int fwd_single_error_flag(bool clear);
-// drafted tokens, head dims 64 and 128 (tree_sm100.cu)
+// drafted tokens, head dims up to 128 (tree_sm100.cu)
 int launch_tree_sm100(const fa_fwd_params& p, const Sm100FwdArgs& a, bool dual);
 int tree_sm100_error_flag(bool clear);
 

@@ -209,7 +209,7 @@ void plan_tree(const fa_fwd_params& p, TreePlan& plan) {
         // a call that asks for n splits gets shares of at least that part of the longest sequence
         if (p.num_splits > 0) plan.min_keys = (int)((((long)p.sk + 127) / 128 + p.num_splits - 1) / p.num_splits) * 128;
         const size_t pieces = plan.shares == 1 ? 0 : (size_t)lanes_of(p) * plan.shares * 2 * (rows <= 128 ? 128 : 256);
-        plan.lse = plan.o + align256(pieces * p.d * 4);
+        plan.lse = plan.o + align256(pieces * (p.d <= 64 ? 64 : 128) * 4);      // partials have the kernel's head dim
         plan.total = plan.lse + align256(pieces * 4);
         return;
     }

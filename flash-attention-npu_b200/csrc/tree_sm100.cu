@@ -1,4 +1,4 @@
-// Attention of drafted tokens over a cache on the tcgen05 tensor cores, head dims 64 and 128, sm_100a.
+// Attention of drafted tokens over a cache on the tcgen05 tensor cores, head dims up to 128, sm_100a.
 //
 // What the two-tile forward (fwd_sm100.cu) does for a block of queries, for the stacked rows of a KV head (tree_mask.cuh), with
 // the work laid out for a cache that has to be streamed once: lengths in a batch differ by factors, they are on the device, and
@@ -219,8 +219,8 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
         // The first tiles are on their way while the other warps arrive and the preparing kernel still runs: those in front of
         // the draft, which it does not write.  A lane has one box of one tile, so that the page table is looked up once.
         const int from = walk.lo + walk.first_tile();
-        ahead = max(0, min(NST, min(walk.count(), walk.L / 128 - from)));
-        const int parts = 128 / a.kv_box, tile = lane / parts, part_of = lane % parts;      // 8 parts at most, 3 tiles
+        const int parts = 128 / a.kv_box, tile = lane / parts, part_of = lane % parts;      // up to 16 parts
+        ahead = max(0, min(min(NST, 32 / parts), min(walk.count(), walk.L / 128 - from)));
         const bool busy = tile < ahead;
         int2 box = make_int2(0, 0);
         if (busy) box = tree_box(a, from * 128 + lane * a.kv_box, walk.b);
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
                     pk.y = Elem<T>::pack(__uint_as_float(oreg[8 * v + 2]) * inv, __uint_as_float(oreg[8 * v + 3]) * inv);
                     pk.z = Elem<T>::pack(__uint_as_float(oreg[8 * v + 4]) * inv, __uint_as_float(oreg[8 * v + 5]) * inv);
                     pk.w = Elem<T>::pack(__uint_as_float(oreg[8 * v + 6]) * inv, __uint_as_float(oreg[8 * v + 7]) * inv);
-                    reinterpret_cast<uint4*>(orow + c * 32)[v] = pk;
+                    if (c * 32 + v * 8 < a.d) reinterpret_cast<uint4*>(orow + c * 32)[v] = pk;
                 }
             }
         }
@@ -584,52 +584,78 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
 }
 
 // Rows whose sequence was cut: its pieces in shares c0 .. c1, joined in that order.  A CTA has 32 rows of a lane, a thread D / 8
-// columns of one of them (32 or 16 bytes of the result), in all pieces.
+// columns of one of them (32 or 16 bytes of the result).  PHASES = 1: a warp has D / 8 columns, in all pieces.  PHASES = 8: few
+// rows, whose sequences may be cut into a piece an SM: a CTA has D / 8 columns, and its warps share out the pieces (B1 T16 H8/1
+// D128, 30000 rows in 120 pieces: whole call 90 us without, 30 with).
 constexpr int kCombineRows = 32;
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, int PHASES>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Sm100FwdArgs a) {
     constexpr int N = D / 32;                                // groups of four columns a thread
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows_all = a.sq * a.gq, blocks = (rows_all + kCombineRows - 1) / kCombineRows;
-    const int hk = blockIdx.x / blocks % a.hkv, b = blockIdx.x / blocks / a.hkv;
+    const int id = PHASES == 1 ? blockIdx.x : blockIdx.x / 8, cols = PHASES == 1 ? warp : blockIdx.x % 8, phase = PHASES == 1 ? 0 : warp;
+    const int hk = id / blocks % a.hkv, b = id / blocks / a.hkv;
     int before, total, L, lo;
     count_entries(a, b, lane, before, total);
     const int n = tiles_of(a, b, L, lo), share = tree_share(total, a.tree_shares, a.min_split_tiles), begin = before + kTurn;
     const int c0 = n ? begin / share : 0, c1 = n ? (begin + n - 1) / share : -1;
     grid_wait_for_previous();
-    const int row = blockIdx.x % blocks * kCombineRows + lane, lanes = a.hkv * a.tree_blocks;
-    if (c0 == c1 || row >= rows_all) return;                 // c0 == c1: finished by its CTA
+    if (c0 == c1) return;                                    // finished by its CTA
+    const int row = id % blocks * kCombineRows + lane, lanes = a.hkv * a.tree_blocks;
     const int mine = hk * a.tree_blocks + row / ROWS;
     float m = -INFINITY, tot = 0.f;
     float4 acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-    for (int c = c0; c <= c1; ++c) {
-        // the piece in share c: the CTA's last one where the sequence begins in its share, else its first
-        const int64_t piece = (int64_t)(c * lanes + mine) * 2 + (c == c0 ? 1 : 0);
-        const float w = __ldcg(a.lse_part + piece * ROWS + row % ROWS);
-        float4 v[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(a.o_part) + (piece * (D / 4) + warp * N + i) * ROWS + row % ROWS);
-        if (w == -INFINITY) continue;                        // a piece in which the row sees nothing
+    auto add = [&](float w, float t, const float4 (&v)[N]) { // a result of weight t e^w
+        if (w == -INFINITY) return;                          // a piece in which the row sees nothing
         const float next = fmaxf(m, w), f = expf(m - next), e = expf(w - next);
         m = next;
-        tot = tot * f + e;
+        tot = tot * f + t * e;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             acc[i].x = acc[i].x * f + e * v[i].x; acc[i].y = acc[i].y * f + e * v[i].y;
             acc[i].z = acc[i].z * f + e * v[i].z; acc[i].w = acc[i].w * f + e * v[i].w;
         }
+    };
+    if (row < rows_all) {
+#pragma unroll 2
+        for (int c = c0 + phase; c <= c1; c += PHASES) {
+            // the piece in share c: the CTA's last one where the sequence begins in its share, else its first
+            const int64_t piece = (int64_t)(c * lanes + mine) * 2 + (c == c0 ? 1 : 0);
+            const float w = __ldcg(a.lse_part + piece * ROWS + row % ROWS);
+            float4 v[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(a.o_part) + (piece * (D / 4) + cols * N + i) * ROWS + row % ROWS);
+            add(w, 1.f, v);
+        }
     }
+    if constexpr (PHASES > 1) {
+        __shared__ float s_m[PHASES][32], s_tot[PHASES][32];
+        __shared__ float4 s_acc[PHASES][N][32];
+        s_m[phase][lane] = m;
+        s_tot[phase][lane] = tot;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s_acc[phase][i][lane] = acc[i];
+        __syncthreads();
+        if (phase) return;
+        for (int k = 1; k < PHASES; ++k) {
+            float4 v[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = s_acc[k][i][lane];
+            add(s_m[k][lane], s_tot[k][lane], v);
+        }
+    }
+    if (row >= rows_all) return;
     const float inv = tot > 0.f ? 1.f / tot : 0.f;
     const int qi = row / a.gq, head = hk * a.gq + row % a.gq;
-    T* orow = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_sb + (int64_t)qi * a.o_ss + (int64_t)head * a.o_sh + warp * N * 4;
+    T* orow = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_sb + (int64_t)qi * a.o_ss + (int64_t)head * a.o_sh + cols * N * 4;
 #pragma unroll
     for (int i = 0; i < N; i += 2)
-        reinterpret_cast<uint4*>(orow)[i / 2] = make_uint4(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv),
-                                                           Elem<T>::pack(acc[i + 1].x * inv, acc[i + 1].y * inv), Elem<T>::pack(acc[i + 1].z * inv, acc[i + 1].w * inv));
-    if (warp == 0 && a.lse)
+        if ((cols * N + i) * 4 < a.d)
+            reinterpret_cast<uint4*>(orow)[i / 2] = make_uint4(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv),
+                                                               Elem<T>::pack(acc[i + 1].x * inv, acc[i + 1].y * inv), Elem<T>::pack(acc[i + 1].z * inv, acc[i + 1].w * inv));
+    if (cols == 0 && a.lse)
         a.lse[(int64_t)b * a.lse_sb + (int64_t)head * a.lse_sh + (int64_t)qi * a.lse_ss] = tot > 0.f ? m + logf(tot) : INFINITY;
 }
 
@@ -641,14 +667,18 @@ int launch_t(const fa_fwd_params& p, const Sm100FwdArgs& a) {
     if (int e = cuda_ok(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute")) return e;
     if (int e = cuda_ok(launch_early(kern, dim3((unsigned)(a.hkv * a.tree_blocks * a.tree_shares)), 384, smem, st, a), "tree_sm100 launch")) return e;
     mark_kernel(st);
+    constexpr int ROWS = DUAL ? 128 : 256;
     const int64_t blocks = (int64_t)p.b * p.hkv * ((p.sq * a.gq + kCombineRows - 1) / kCombineRows);
-    if (int e = cuda_ok(launch_early(tree_combine_kernel<T, D, DUAL ? 128 : 256>, dim3((unsigned)blocks), 256, 0, st, a), "tree_combine launch")) return e;
+    // fewer blocks than two an SM: each is made eight
+    const cudaError_t e = blocks < 2 * sm_count() ? launch_early(tree_combine_kernel<T, D, ROWS, 8>, dim3((unsigned)blocks * 8), 256, 0, st, a)
+                                                  : launch_early(tree_combine_kernel<T, D, ROWS, 1>, dim3((unsigned)blocks), 256, 0, st, a);
+    if (int code = cuda_ok(e, "tree_combine launch")) return code;
     mark_kernel(st);
     return FA_OK;
 }
 template <typename T>
 int launch_dims(const fa_fwd_params& p, const Sm100FwdArgs& a, bool dual) {
-    if (p.d == 128) return dual ? launch_t<T, 128, true>(p, a) : launch_t<T, 128, false>(p, a);
+    if (p.d > 64) return dual ? launch_t<T, 128, true>(p, a) : launch_t<T, 128, false>(p, a);
     return dual ? launch_t<T, 64, true>(p, a) : launch_t<T, 64, false>(p, a);
 }
 

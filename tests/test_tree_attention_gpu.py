@@ -135,6 +135,10 @@ def test_missing_tokens_are_neither_written_nor_seen(layout):
     c = make(_T[dt], d, hq, hkv, lens, t, page, seed=7 * d + t, holes=0.25, ragged=True, rotary="half")
     c["k"][c["parents"] < -1], c["v"][c["parents"] < -1] = float("nan"), float("inf")
     check(c)
+    c["q"][c["parents"] < -1] = float("nan")
+    check(c)
+    check(c, softcap=8.0)
+    check(c, num_splits=2)
 
 
 @pytest.mark.parametrize("t", [1, 2, 31, 32, 33, 65])
@@ -293,8 +297,9 @@ def test_depths_of_the_reference():
 
 @pytest.mark.parametrize("d,softcap,page,hq,t,name,form", [
     (128, 0.0, 64, 8, 16, "sm100_tcgen05_tree", 1), (64, 0.0, 16, 14, 40, "sm100_tcgen05_tree", 0), (128, 20.0, 0, 6, 9, "sm100_tcgen05_2q", 2),
-    (256, 0.0, 32, 4, 9, "sm100_tcgen05_wide", 0), (192, 5.0, 128, 4, 9, "sm100_tcgen05_wide", 0), (96, 0.0, 64, 4, 9, "generic_mma", 0),
-    (128, 0.0, 48, 8, 16, "sm100_tcgen05_tree", 1), (128, 0.0, 40, 8, 16, "generic_mma", 0)])
+    (256, 0.0, 32, 4, 9, "sm100_tcgen05_wide", 0), (192, 5.0, 128, 4, 9, "sm100_tcgen05_wide", 0), (96, 0.0, 64, 4, 9, "sm100_tcgen05_tree", 1), (224, 0.0, 64, 4, 9, "sm100_tcgen05_wide", 0),
+    (40, 9.0, 16, 8, 20, "sm100_tcgen05_2q", 2),
+    (128, 0.0, 48, 8, 16, "sm100_tcgen05_tree", 1), (128, 0.0, 40, 8, 16, "sm100_tcgen05_tree", 1), (128, 0.0, 36, 8, 16, "generic_mma", 0), (72, 0.0, 1, 8, 16, "generic_mma", 0)])
 def test_which_kernel_runs(d, softcap, page, hq, t, name, form):
     check(make(torch.bfloat16, d, hq, 2, [150, 300], t, page, seed=d + page), softcap=softcap)
     assert capi.last_kernel() == name and capi.lib.fa_debug_get(8) == form
@@ -318,6 +323,8 @@ def test_the_general_kernels_agree():
     (4, 1, 200, [700, 90]),
     (2, 2, 3, [12000]),                                   # one sequence over many CTAs
     (16, 16, 2, [40, 700] * 20),                          # 640 units
+    (8, 1, 16, [20000]),                                  # ... an SM each: pieces shared out to the warps that join them
+    (8, 1, 31, [9000, 11, 7000]),
 ])
 @pytest.mark.parametrize("left", [-1, 100])
 def test_shares_of_the_key_tiles(hq, hkv, t, lens, left):
@@ -328,3 +335,24 @@ def test_shares_of_the_key_tiles(hq, hkv, t, lens, left):
 def test_many_sequences():
     """More sequences than one step of the search for a CTA's first one looks at."""
     check(make(torch.bfloat16, 64, 2, 1, [(37 * i) % 300 for i in range(1100)], 2, 64, seed=3))
+
+
+@pytest.mark.parametrize("d", [40, 72, 96, 120])
+def test_workspace_has_room_for_padded_head_dims(d):
+    """The pieces of cut sequences have the kernel's head dim, 64 or 128, whatever the call's is."""
+    def need(dim):
+        t = capi.TreeParams()
+        p = t.fwd
+        p.dtype, p.b, p.sq, p.sk, p.hq, p.hkv, p.d, p.dv, p.scale, p.kv_entries, p.page_size = 1, 16, 26, 8192, 32, 8, dim, dim, 0.1, 999, 64
+        p.block_table, p.window_left = 0x1000, -1
+        for x in (p.k, p.v):
+            x.stride_b, x.stride_s, x.stride_h = 1 << 20, 8 * dim, dim
+        return capi.lib.fa_tree_workspace_bytes(t), 16 * 26 * 32 * dim * 2
+    full, queries = need(64 if d <= 64 else 128)
+    got, fewer = need(d)
+    assert got - fewer >= full - queries - 256
+
+
+def test_padded_head_dim_over_many_pieces():
+    check(make(torch.bfloat16, 96, 8, 4, [3000, 1700, 40, 2500], 26, 64, seed=17))
+    check(make(torch.float16, 40, 16, 2, [2600, 900], 30, 16, seed=18))
