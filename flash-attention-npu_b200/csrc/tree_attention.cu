@@ -165,8 +165,8 @@ struct TreePlan {
 };
 
 // tree_sm100.cu: lanes (row blocks of KV heads), and into how many shares the list of key tiles is cut.  All CTAs do about the
-// same, so what counts is how many of them an SM gets one after the other: the fewest such rounds a share, one round if that
-// leaves no more than a twelfth of the SMs without work.
+// same and an SM holds one, so a call takes as long as its rounds of CTAs, each 1 / n of the list; a round also costs its start
+// and its ends, put at 8 % of what the call takes at best.  8 lanes: 18 shares (144 of 148 SMs); 40 lanes: 7 (two rounds).
 long lanes_of(const fa_fwd_params& p) {
     const long rows = (long)p.sq * (p.hq / p.hkv);
     return p.hkv * (rows <= 128 ? 1 : (rows + 255) / 256);

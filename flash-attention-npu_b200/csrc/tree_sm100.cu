@@ -8,7 +8,9 @@
 // neighbours in the grid: they read the heads of the same cache rows, or the same rows, at the same time.  A sequence that lies
 // in one share is finished there; one that the shares cut is left in pieces, at most two a CTA (the first and the last of its
 // share), as normalised fp32 partials that tree_combine_kernel joins in order.  Between sequences the copies of K and V run on.
-// B8, 64 tokens, up to 32768 rows, H32/8 D128: 183 us with a CTA a split, see below for now.
+// Whole calls, graph replays, H32/8 D128: 64 tokens x 8 sequences up to 32768 rows 199 us with a CTA a split, 166 so; 26 x 16 up to
+// 8192 rows 93 / 85 (337 MB: 4.0 TB/s; inside a CTA tiles come at the memory's pace, 20 us are start, ends and the two kernels
+// around it).
 //
 // DUAL: lanes of up to 128 rows.  Both softmax groups work on the same rows, group x on key tiles x, x + 2, .. of the piece,
 // and merge their results at its end.  Otherwise group x has rows 128 x .. 128 x + 127 and every tile.
