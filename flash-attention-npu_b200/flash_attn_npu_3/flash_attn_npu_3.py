@@ -179,9 +179,9 @@ def _input(t):
     return t, (ptr, s0, s1, s2)
 
 
-def _wrong_tensor(name, t, dtype, index):
-    capi.cuda_index(t)
-    raise RuntimeError(f"{name} must have the dtype and the device of q")
+def _wrong_tensors(*tensors):
+    capi.require_cuda(*tensors)
+    raise RuntimeError("k, v and the caches must have the dtype and the device of q")
 
 
 def _int32(name, t, index):
@@ -206,9 +206,10 @@ def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cac
     code = capi.DTYPES.get(dtype)
     if code is None:
         raise RuntimeError("FlashAttention only supports FP16 and BF16 data types")
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("k", k), ("v", v)):
-        if t is not None and (t.dtype is not dtype or t.get_device() != index):
-            _wrong_tensor(name, t, dtype, index)
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype or k_cache.get_device() != index or v_cache.get_device() != index:
+        _wrong_tensors(k_cache, v_cache)
+    if k is not None and v is not None and (k.dtype is not dtype or v.dtype is not dtype or k.get_device() != index or v.get_device() != index):
+        _wrong_tensors(k, v)
     if d_cache != d or d % 8 != 0 or d > 256:
         raise RuntimeError("q and the cache must have the same head dimension, a multiple of 8 of at most 256")
     if hkv == 0 or hq % hkv != 0:
@@ -287,7 +288,7 @@ def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cac
         if rotary_positions is not None:
             rotary_positions, st = check_positions(rotary_positions, axes[1], (batch, tokens), index)
             positions = (rotary_positions.data_ptr(), st[0], st[1])
-    out = q.new_empty((batch, tokens, hq, d))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((batch, hq, tokens), dtype=torch.float32)
     if k is not None and (k.shape != (batch, tokens, hkv, d) or v.shape != (batch, tokens, hkv, d)):
         raise RuntimeError(f"k and v must have shape {(batch, tokens, hkv, d)}")

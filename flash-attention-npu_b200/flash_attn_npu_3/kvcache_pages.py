@@ -4,6 +4,7 @@ cache calls take a page table as it is given, flash_attn_npu_3/flash_attn_npu_in
 The pool's state is one int32 reference count a page, `page_refs` (num_pages,), zeros to begin with; a page is free when its
 count is 0.  Page tables are int32 (batch, max_pages), filled from the left, -1 where there is no page.  Everything stays on
 the device and on the current stream: no call waits for the host, and each can be captured into a CUDA graph."""
+import functools
 import struct
 from typing import Optional
 
@@ -124,8 +125,13 @@ def _run(fn, index, views, num_caches, num_pages, page_size, refs, table, table_
     capi.launch_on(fn, buf, index)
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_ints(rows, num_pages):
+    return (capi.lib.fa_pages_workspace_bytes(rows, num_pages) + 3) // 4
+
+
 def _workspace(like, rows, num_pages):
-    return like.new_empty((capi.lib.fa_pages_workspace_bytes(rows, num_pages) + 3) // 4)
+    return like.new_empty(_workspace_ints(rows, num_pages))
 
 
 def kvcache_reserve(page_refs, page_table, cache_seqlens, page_size, extra=0):
@@ -181,7 +187,7 @@ def kvcache_fork(caches, page_refs, page_table, cache_seqlens, parents, keep_par
     if not parents.is_contiguous():
         parents = parents.contiguous()
     new_table = page_refs.new_empty((n, width))
-    new_lens, missing = page_refs.new_empty(n), page_refs.new_empty(1)
+    new_lens, missing = torch.empty_like(parents), page_refs.new_empty(1)
     _run(capi._call_fork, index, views, num, pages, page_size, page_refs, table, stride, b, width, 0, n, 1 if keep_parents else 0, lens, parents,
          None, 0, None, new_table, new_lens, missing, _workspace(page_refs, n, pages))
     return new_table, new_lens, missing
@@ -223,7 +229,7 @@ def kvcache_compact(caches, cache_seqlens, kept, counts: Optional[torch.Tensor] 
         cache_batch_idx = _row("cache_batch_idx", cache_batch_idx, b, index)
     elif entries < b:
         raise RuntimeError("the caches have fewer entries than the batch")
-    out = lens.new_empty(b)
+    out = torch.empty_like(lens)
     _run(capi._call_compact, index, views, num, entries, rows, None, table, stride, b, width, 0, n, 0, lens, kept, counts, kept_stride,
          cache_batch_idx, None, out, None)
     return out

@@ -77,7 +77,7 @@ def _run(q, k, cos, sin, positions, sections, cyclic, interleaved, backward, inp
     pos = positions.stride()
     if len(pos) == len(shape) - 2:
         pos = (0,) + pos
-    q_out = q if inplace else q.new_empty(shape)
+    q_out = q if inplace else torch.empty_like(q, memory_format=torch.contiguous_format)
     dense = (s * hq * d, hq * d, d)
     q_in = _leaves(q, st)
     q_to = q_in if inplace else (q_out.data_ptr(),) + dense
@@ -88,7 +88,7 @@ def _run(q, k, cos, sin, positions, sections, cyclic, interleaved, backward, inp
             k = k.contiguous()
             st = k.stride()
         hk = k.shape[-2]
-        k_out = k if inplace else k.new_empty(k.shape)
+        k_out = k if inplace else torch.empty_like(k, memory_format=torch.contiguous_format)
         k_in = _leaves(k, st)
         k_to = k_in if inplace else (k_out.data_ptr(), s * hk * d, hk * d, d)
     if b * s * (hq + hk) > 0:
@@ -119,7 +119,7 @@ def _rotary_axes_fake(q, k, cos, sin, positions, sections, cyclic, interleaved, 
 
 
 def _forward(q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
-    if capi.plain(q, k, cos, sin, positions):                  # the op's dispatch would do nothing but call the body
+    if capi.plain(q, k, cos):                                  # the op's dispatch would do nothing but call the body
         return _out_of_place(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
     q_out, k_out = _rotary_axes(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
     return q_out, None if k is None else k_out
@@ -166,7 +166,7 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
     i belongs to axis i % axes while that axis has pairs left, else to axis 0.  None: one axis.  A position outside the tables
     takes the nearest row.  fp32 arithmetic, rounded once; cos, sin and positions get no gradient.
 
-    inplace writes into q and k instead of new tensors (only where no gradient is needed).
+    inplace writes into q and k instead of new tensors (only where no gradient is needed); q and k must not share memory.
     Returns (q, k), or q alone when k is None."""
     index, dtype, shape = capi.cuda_index(q), q.dtype, q.shape
     if dtype not in capi.DTYPES or (k is not None and k.dtype is not dtype):
@@ -174,15 +174,13 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
     n = len(shape)
     if n != 3 and n != 4:
         raise RuntimeError("q must be (batch, seqlen, nheads, headdim) or (total, nheads, headdim)")
-    lead = shape[:-2]
     if k is not None:
         other = k.shape
-        if len(other) != n or other[:-2] != lead or other[-1] != shape[-1]:
+        if len(other) != n or other[0] != shape[0] or other[-3] != shape[-3] or other[-1] != shape[-1]:
             raise RuntimeError("k must have the shape of q but for its heads")
-    for t in (k, cos, sin):
-        if t is not None and t.get_device() != index:
-            capi.cuda_index(t)
-            raise RuntimeError("q, k, cos and sin must be on one device")
+    if cos.get_device() != index or sin.get_device() != index or (k is not None and k.get_device() != index):
+        capi.require_cuda(k, cos, sin)
+        raise RuntimeError("q, k, cos and sin must be on one device")
     table = cos.shape
     if len(table) != 2 or sin.shape != table or sin.dtype is not cos.dtype or (cos.dtype is not dtype and cos.dtype is not torch.float32):
         raise RuntimeError("cos and sin must both have shape (seqlen_ro, rotary_dim / 2), in q's dtype or fp32")
@@ -190,10 +188,12 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
     if d > 256 or d % 2 or not 0 < 2 * pairs <= d or rows == 0:
         raise RuntimeError("the head dimension must be even and at most 256, rotary_dim positive and at most that, with one table row at least")
     sections_cyclic = bool(sections_cyclic)
+    axes = 1
     if sections is not None:
         sections = list(sections)
+        axes = len(sections)
         axis_table(pairs, tuple(sections), sections_cyclic)
-    positions, _ = check_positions(positions, 1 if sections is None else len(sections), lead, index)
+    positions, _ = check_positions(positions, axes, shape[:-2], index)
     if not cos.is_contiguous() or not sin.is_contiguous():
         cos, sin = cos.contiguous(), sin.contiguous()
     args = (cos, sin, positions, sections, sections_cyclic, bool(interleaved))
@@ -205,7 +205,10 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
                 raise RuntimeError("inplace rotary embedding is not differentiable: detach q and k, or leave inplace out")
             if t.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise RuntimeError("inplace rotary embedding needs a contiguous last dimension and no expanded dimensions")
+        if k is not None and k.data_ptr() == q.data_ptr() and k.numel():
+            raise RuntimeError("inplace rotary embedding needs q and k in memory of their own")
         _run(q, k, *args, False, True)
+        torch.autograd.graph.increment_version(q if k is None else (q, k))
     else:
         q, k = _apply(q, k, *args, False)
     return q if k is None else (q, k)

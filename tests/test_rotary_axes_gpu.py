@@ -95,7 +95,7 @@ def test_forward_backward_and_in_place(case):
     with torch.no_grad():
         qi, ki = q.detach().clone(), k.detach().clone()
         r = fa.rotary_axes_func(qi, ki, cos, sin, pos, inplace=True, **kw)
-        assert r[0] is qi and r[1] is ki
+        assert r[0] is qi and r[1] is ki and qi._version == 1 and ki._version == 1
         assert torch.equal(qi.view(torch.int16), qo.view(torch.int16)) and torch.equal(ki.view(torch.int16), ko.view(torch.int16))
         alone = fa.rotary_axes_func(q, None, cos, sin, pos, **kw)
         assert torch.equal(alone.view(torch.int16), qo.view(torch.int16))
@@ -209,6 +209,18 @@ def test_refusals(change, word):
         dev[k] = x[:, :, :1].cuda().expand(x.shape) if expanded else x.detach().cuda().requires_grad_(x.requires_grad) if isinstance(x, torch.Tensor) else x
     with pytest.raises(RuntimeError, match=word):
         fa.rotary_axes_func(**dev)
+
+
+@pytest.mark.gpu
+def test_in_place_on_one_tensor_twice_or_on_what_a_gradient_needs():
+    q, _, cos, sin, pos = inputs(torch.bfloat16, (2, 4), 4, 4, 64, 64, 1, torch.float32)
+    with pytest.raises(RuntimeError, match="memory of their own"):
+        fa.rotary_axes_func(q, q, cos, sin, pos, inplace=True)
+    x = torch.randn_like(q).requires_grad_(True)
+    y = (x * q).sum()                                            # keeps q for dx
+    fa.rotary_axes_func(q, None, cos, sin, pos, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
 
 
 def test_c_entry_point_refusals():
