@@ -50,19 +50,25 @@ __device__ __forceinline__ RotaryRows same_row(const RotaryAxes& r, int pos) {
 template <typename TT> __device__ __forceinline__ float table_value(const TT* t) { return Elem<TT>::to_float(*t); }
 template <> __device__ __forceinline__ float table_value<float>(const float* t) { return *t; }
 
-// cosines and sines of pairs i0 .. i0 + 7 (i0 a multiple of 8): 16-byte loads where one axis turns all of them
-template <typename TT>
-__device__ __forceinline__ void load_angles8(const RotaryAxes& r, const RotaryRows& p, int i0, float (&c)[8], float (&s)[8]) {
+// Chunks of W elements, moved at once: 16 bytes, or 8 where rotary_dim / 2 is a multiple of 4 only
+template <int W> struct ChunkOf;
+template <> struct ChunkOf<8> { using type = uint4; };
+template <> struct ChunkOf<4> { using type = uint2; };
+
+// cosines and sines of pairs i0 .. i0 + W - 1 (i0 a multiple of W): wide loads where one axis turns all of them
+template <typename TT, int W = 8>
+__device__ __forceinline__ void load_angles(const RotaryAxes& r, const RotaryRows& p, int i0, float (&c)[W], float (&s)[W]) {
     const TT* cos = reinterpret_cast<const TT*>(r.cos);
     const TT* sin = reinterpret_cast<const TT*>(r.sin);
     const int half = r.rd / 2;
-    const uint32_t axes = (r.axis[i0 >> 4] >> ((i0 & 15) * 2)) & 0xffffu;
-    if (axes == (axes & 3) * 0x5555u) {
+    const uint32_t axes = (r.axis[i0 >> 4] >> ((i0 & 15) * 2)) & ((1u << 2 * W) - 1u);
+    if (axes == (axes & 3) * (0x5555u & ((1u << 2 * W) - 1u))) {
         const int64_t at = (int64_t)p.of(axes & 3) * half + i0;
-        constexpr int N = 16 / sizeof(TT);
+        constexpr int N = W * sizeof(TT) < 16 ? W : 16 / sizeof(TT);
+        using V = typename ChunkOf<N * sizeof(TT) / 2>::type;
 #pragma unroll
-        for (int k = 0; k < 8; k += N) {
-            const uint4 vc = *reinterpret_cast<const uint4*>(cos + at + k), vs = *reinterpret_cast<const uint4*>(sin + at + k);
+        for (int k = 0; k < W; k += N) {
+            const V vc = *reinterpret_cast<const V*>(cos + at + k), vs = *reinterpret_cast<const V*>(sin + at + k);
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 c[k + e] = table_value<TT>(reinterpret_cast<const TT*>(&vc) + e);
@@ -71,7 +77,7 @@ __device__ __forceinline__ void load_angles8(const RotaryAxes& r, const RotaryRo
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < W; ++e) {
             const int64_t at = (int64_t)p.of((axes >> (2 * e)) & 3) * half + i0 + e;
             c[e] = table_value<TT>(cos + at);
             s[e] = table_value<TT>(sin + at);
@@ -82,28 +88,29 @@ __device__ __forceinline__ void turn(float a, float b, float c, float s, float& 
     ya = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
     yb = __fadd_rn(__fmul_rn(a, s), __fmul_rn(b, c));
 }
-// Unit u of a head's row: the two 8-element chunks that hold pairs 8 u .. 8 u + 7.  lo, hi: chunk numbers
+// Unit u of a head's row: the two W-element chunks that hold pairs W u .. W u + W - 1.  lo, hi: chunk numbers
+template <int W = 8>
 __device__ __forceinline__ void unit_chunks(const RotaryAxes& r, int u, int& lo, int& hi) {
-    const bool apart = u < r.rd / 16 && !r.interleaved;
+    const bool apart = u < r.rd / (2 * W) && !r.interleaved;
     lo = apart ? u : 2 * u;
-    hi = apart ? u + r.rd / 16 : 2 * u + 1;
+    hi = apart ? u + r.rd / (2 * W) : 2 * u + 1;
 }
-template <typename T>
-__device__ __forceinline__ void turn8(const uint4 a, const uint4 b, const float (&c)[8], const float (&s)[8], bool interleaved, uint4& ya, uint4& yb) {
+template <typename T, int W = 8, typename C = typename ChunkOf<W>::type>
+__device__ __forceinline__ void turn_chunks(const C a, const C b, const float (&c)[W], const float (&s)[W], bool interleaved, C& ya, C& yb) {
     const T *xa = reinterpret_cast<const T*>(&a), *xb = reinterpret_cast<const T*>(&b);
     uint32_t *oa = reinterpret_cast<uint32_t*>(&ya), *ob = reinterpret_cast<uint32_t*>(&yb);
     if (interleaved) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < W / 2; ++e) {
             float p, q;
             turn(Elem<T>::to_float(xa[2 * e]), Elem<T>::to_float(xa[2 * e + 1]), c[e], s[e], p, q);
             oa[e] = Elem<T>::pack(p, q);
-            turn(Elem<T>::to_float(xb[2 * e]), Elem<T>::to_float(xb[2 * e + 1]), c[4 + e], s[4 + e], p, q);
+            turn(Elem<T>::to_float(xb[2 * e]), Elem<T>::to_float(xb[2 * e + 1]), c[W / 2 + e], s[W / 2 + e], p, q);
             ob[e] = Elem<T>::pack(p, q);
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
+        for (int e = 0; e < W; e += 2) {
             float p0, q0, p1, q1;
             turn(Elem<T>::to_float(xa[e]), Elem<T>::to_float(xb[e]), c[e], s[e], p0, q0);
             turn(Elem<T>::to_float(xa[e + 1]), Elem<T>::to_float(xb[e + 1]), c[e + 1], s[e + 1], p1, q1);
@@ -112,7 +119,7 @@ __device__ __forceinline__ void turn8(const uint4 a, const uint4 b, const float 
         }
     }
 }
-// element e of a head's row, for rotary dims that are no multiple of 16 and tables that are not 16-byte aligned
+// element e of a head's row, for other rotary dims and tables that are not aligned
 template <typename T, typename TT>
 __device__ __forceinline__ T turn_elem(const T* x, int e, const RotaryAxes& r, const RotaryRows& p, float sign) {
     if (e >= r.rd) return x[e];

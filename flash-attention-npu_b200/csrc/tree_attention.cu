@@ -143,9 +143,9 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
             int lo, hi;
             unit_chunks(a.ro, u, lo, hi);
             float c[8], s[8];
-            load_angles8<T>(a.ro, rows, u * 8, c, s);
+            load_angles<T>(a.ro, rows, u * 8, c, s);
             uint4 ya, yb;
-            turn8<T>(s4[lo], s4[hi], c, s, a.ro.interleaved, ya, yb);
+            turn_chunks<T>(s4[lo], s4[hi], c, s, a.ro.interleaved, ya, yb);
             d4[lo] = ya;
             d4[hi] = yb;
         } else {

@@ -59,7 +59,12 @@ CASES = [  # dtype, lead, hq, hk, d, rd, axes, cyclic, interleaved, fp32 tables
     ("bf16", (1, 1), 32, 8, 128, 128, 1, False, True, True),
     ("bf16", (3, 33), 7, 1, 256, 256, 4, True, True, False),
     ("fp16", (2, 9), 5, 3, 96, 48, 2, False, False, True),
-    ("bf16", (2, 9), 5, 3, 80, 40, 2, False, False, True),       # rotary dim no multiple of 16: element by element
+    ("bf16", (2, 9), 5, 3, 80, 40, 2, False, False, True),       # rotary dim no multiple of 16: four elements at once
+    ("fp16", (31,), 6, 1, 128, 40, 3, False, True, False),
+    ("bf16", (3, 5), 8, 2, 256, 72, 2, True, False, True),
+    ("fp16", (9,), 4, 2, 60, 24, 3, False, False, False),         # a row ends inside a unit
+    ("bf16", (2, 6), 2, 1, 20, 16, 1, False, True, True),
+    ("fp16", (5,), 3, 2, 72, 20, 2, False, False, True),         # element by element
     ("fp16", (11,), 3, 2, 72, 22, 3, False, True, False),
     ("bf16", (4, 3), 2, 2, 50, 34, 1, False, False, True),       # head dim no multiple of 8
     ("bf16", (700,), 16, 16, 64, 32, 3, True, True, True),
