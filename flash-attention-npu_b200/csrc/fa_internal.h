@@ -64,6 +64,7 @@ int launch_fwd_generic(const fa_fwd_params& p, const FwdPlan& plan, float* o_par
 struct TreeMask;                                     // tree_mask.cuh
 bool fwd_sm100_tree_supported(const fa_fwd_params& p);
 long fwd_sm100_tree_ctas(const fa_fwd_params& p);     // CTAs of one key split
+int fwd_sm100_tree_resident(const fa_fwd_params& p); // of them on an SM
 bool fwd_sm100_tree_shared(const fa_fwd_params& p);  // runs on the kernel that shares out the key tiles itself: no splits
 int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, int shares, float* o_part, float* lse_part);
 int launch_fwd_generic_tree(const fa_fwd_params& p, const TreeMask& tree, int nsplit, int min_split_keys, float* o_part, float* lse_part);

@@ -192,8 +192,13 @@ void plan_tree(const fa_fwd_params& p, TreePlan& plan) {
     plan.min_keys = plan.shared ? 256 : 512;
     const long base = plan.sm100 ? fwd_sm100_tree_ctas(p) : (long)p.b * p.hkv * ((rows + kGenericBM - 1) / kGenericBM);
     const long most = ((long)p.sk + plan.min_keys - 1) / plan.min_keys;
+    // Splits of the kernels that do not share out the tiles: as many as run side by side, where that is enough of them, else two
+    // rounds of CTAs (four of the generic kernel's), whose rest falls on SMs that short sequences left.  Head dim 256, one CTA an
+    // SM, 5 / 8 / 12 / 16 sequences of 8 heads: 3 splits 81 us (8: 106), 2 96 (5: 109), 4 111 (1: 130), 3 140 (1: 165); capped at
+    // head dim 128, two CTAs an SM: 7 59 (8: 78), 4 74 (5: 86), 3 79 (7: 81), 5 105 (2: 122)
+    const long resident = plan.sm100 ? fwd_sm100_tree_resident(p) : 1, slots = resident * sm_count();
     const long waves = plan.sm100 ? 2 : 4;
-    long n = p.num_splits > 0 ? p.num_splits : (waves * sm_count() + base - 1) / base;
+    long n = p.num_splits > 0 ? p.num_splits : plan.sm100 && base * (resident + 1) <= slots ? slots / base : (waves * slots + base - 1) / base;
     if (n > most) n = most;
     if (n > 256) n = 256;
     if (n > 65535 / p.b) n = 65535 / p.b;
