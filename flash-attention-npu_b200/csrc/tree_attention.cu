@@ -174,10 +174,11 @@ long lanes_of(const fa_fwd_params& p) {
 int shares_of(const fa_fwd_params& p) {
     const long lanes = lanes_of(p), sms = sm_count();
     long best = 1;
-    double best_cost = 0;
-    for (long n = 1; n <= 8 * sms && (n == 1 || n * lanes <= 3 * sms); ++n) {
-        const double rounds = (double)((n * lanes + sms - 1) / sms), cost = rounds / n + 0.08 * rounds * lanes / sms;
-        if (n == 1 || cost < best_cost) { best = n; best_cost = cost; }
+    double best_cost = (double)((lanes + sms - 1) / sms) * (1. + 0.08 * lanes / sms);
+    for (int rounds = 1; rounds <= 3; ++rounds) {            // the most shares that so many rounds have room for
+        const long n = rounds * sms / lanes;
+        const double cost = n ? rounds * (1. / n + 0.08 * lanes / sms) : best_cost;
+        if (cost < best_cost) { best = n; best_cost = cost; }
     }
     return (int)best;
 }
