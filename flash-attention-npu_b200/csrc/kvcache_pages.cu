@@ -526,6 +526,7 @@ int run_reserve(const fa_pages_params& p) {
     if (int e = check_table(p, true)) return e;
     if (p.b > 0 && !p.seqlens) return fail(FA_ERR_NULL, "cache_seqlens is null");
     if (!p.missing) return fail(FA_ERR_NULL, "missing is null");
+    if ((int64_t)p.b * p.width > 0x7fffffff) return fail(FA_ERR_BAD_SHAPE, "the page table is too large");   // needs are summed in 32 bits
     if (int e = check_workspace(p, p.b)) return e;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(p.stream);
     PoolArgs a = pool_args(p);

@@ -380,7 +380,7 @@ def flash_attn_tree_with_kvcache(q, k_cache, v_cache, k, v, tree_parents,
     headdim) or paged (num_pages, page_size, nheads_k, headdim) with an int32 page_table (batch, max_pages), as in
     flash_attn_with_kvcache.  cache_seqlens (int or int32 (batch,)): the rows in front of the draft.  k, v (batch, tokens,
     nheads_k, headdim) are written into the cache IN PLACE at rows cache_seqlens .. cache_seqlens + tokens - 1; None when they
-    stand there already.
+    stand there already.  Prefix rows may be shared between sequences, a row that one of them writes may not.
 
     tree_parents (batch, tokens), or (tokens,) for all sequences, int32: the parent of each token, a token in front of it, or
     -1 for a child of the last cached row.  A token attends to all cached rows, its ancestors and itself.  Any other value,

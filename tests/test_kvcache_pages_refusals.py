@@ -31,7 +31,7 @@ def test_null(name):
     ("reserve", {}, 6), ("fork", {}, 6),
     ("reserve", dict(page_size=0), 3), ("reserve", dict(b=-1), 3), ("reserve", dict(num_pages=0), 3), ("reserve", dict(num_pages=1 << 25), 3),
     ("reserve", dict(refs=None), 1), ("reserve", dict(table=None), 1), ("reserve", dict(seqlens=None), 1), ("reserve", dict(missing=None), 1),
-    ("reserve", dict(width=1 << 28), 3), ("reserve", dict(workspace=0x1008, workspace_bytes=1 << 20), 4),
+    ("reserve", dict(width=1 << 28), 3), ("reserve", dict(b=1 << 20, width=1 << 12), 3), ("reserve", dict(workspace=0x1008, workspace_bytes=1 << 20), 4),
     ("free", dict(page_size=-1), 3), ("free", dict(refs=None), 1), ("free", dict(table=None), 1),
     ("fork", dict(rows=None), 1), ("fork", dict(new_table=None), 1), ("fork", dict(new_table=0x1000), 5), ("fork", dict(caches=None), 1), ("fork", dict(n=-1), 3),
     ("copy", dict(rows=None), 1), ("copy", dict(rows2=None), 1), ("copy", dict(num_pages=0), 3), ("copy", dict(n=-1), 3),
