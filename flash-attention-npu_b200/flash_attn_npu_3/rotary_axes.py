@@ -119,7 +119,7 @@ def _rotary_axes_fake(q, k, cos, sin, positions, sections, cyclic, interleaved, 
 
 
 def _forward(q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
-    if capi.plain(q, k, cos):                                  # the op's dispatch would do nothing but call the body
+    if capi.plain(q, k, cos, sin):                             # the op's dispatch would do nothing but call the body
         return _out_of_place(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
     q_out, k_out = _rotary_axes(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
     return q_out, None if k is None else k_out

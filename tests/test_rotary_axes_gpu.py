@@ -217,6 +217,20 @@ def test_refusals(change, word):
 
 
 @pytest.mark.gpu
+def test_tables_from_complex_numbers():
+    """.imag of a conjugate is a lazily negated, strided view: what is read must be the negated values."""
+    q, k, cos, sin, pos = inputs(torch.bfloat16, (2, 4), 4, 2, 64, 64, 1, torch.float32)
+    z = torch.complex(cos, sin).conj()
+    assert z.imag.is_neg()
+    want = fa.rotary_axes_func(q, k, cos, -sin, pos)
+    for tables in ((z.real, z.imag), (cos, torch._neg_view(sin))):
+        got = fa.rotary_axes_func(q, k, *tables, pos)
+        assert all(torch.equal(x, y) for x, y in zip(want, got))
+    here = fa.rotary_axes_func(q.clone(), k.clone(), z.real, z.imag, pos, inplace=True)
+    assert all(torch.equal(x, y) for x, y in zip(want, here))
+
+
+@pytest.mark.gpu
 def test_in_place_on_one_tensor_twice_or_on_what_a_gradient_needs():
     q, _, cos, sin, pos = inputs(torch.bfloat16, (2, 4), 4, 4, 64, 64, 1, torch.float32)
     with pytest.raises(RuntimeError, match="memory of their own"):
