@@ -585,67 +585,100 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
     }
 }
 
-// Rows whose sequence was cut: its pieces in shares c0 .. c1, joined in that order.  A CTA has 32 rows of a lane, a thread D / 8
-// columns of one of them (32 or 16 bytes of the result).  PHASES = 1: a warp has D / 8 columns, in all pieces.  PHASES = 8: few
-// rows, whose sequences may be cut into a piece an SM: a CTA has D / 8 columns, and its warps share out the pieces (B1 T16 H8/1
-// D128, 30000 rows in 120 pieces: whole call 90 us without, 30 with).
+// Rows whose sequence was cut: its pieces in shares c0 .. c1, joined in that order.  A CTA has 32 rows of a lane, a thread 4 N
+// columns of one of them, a warp the same columns of its 32 rows; PHASES warps share out the pieces.
+//   many rows (two CTAs an SM with D / 8 columns a thread)   D / 8 columns: 26 tokens x 16 sequences 83.2 us a call, with 8 columns 85.5
+//   fewer                                                    8 columns: 16 x 8, up to 3000 rows 35.9, with 16 columns 37.1
+//   fewer, 16 shares a sequence or more                      eight warps share out the pieces: one sequence of 30000 rows of two KV
+//                                                            heads 24.6, one warp 31.7; two sequences in 9 shares each 46.5 / 44.1
 constexpr int kCombineRows = 32;
-template <typename T, int D, int ROWS, int PHASES>
+template <typename T, int D, int ROWS, int N, int PHASES>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant__ Sm100FwdArgs a) {
-    constexpr int N = D / 32;                                // groups of four columns a thread
+    constexpr int U = 8 / N;                                 // pieces in flight
+    constexpr int WIDE = 8 / PHASES, SPLIT = D / (4 * N) / WIDE;   // column groups of a CTA, CTAs of the same rows
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows_all = a.sq * a.gq, blocks = (rows_all + kCombineRows - 1) / kCombineRows;
-    const int id = PHASES == 1 ? blockIdx.x : blockIdx.x / 8, cols = PHASES == 1 ? warp : blockIdx.x % 8, phase = PHASES == 1 ? 0 : warp;
+    const int id = blockIdx.x / SPLIT, cols = blockIdx.x % SPLIT * WIDE + warp % WIDE, phase = warp / WIDE;
     const int hk = id / blocks % a.hkv, b = id / blocks / a.hkv;
     int before, total, L, lo;
     count_entries(a, b, lane, before, total);
     const int n = tiles_of(a, b, L, lo), share = tree_share(total, a.tree_shares, a.min_split_tiles), begin = before + kTurn;
     const int c0 = n ? begin / share : 0, c1 = n ? (begin + n - 1) / share : -1;
-    grid_wait_for_previous();
-    if (c0 == c1) return;                                    // finished by its CTA
     const int row = id % blocks * kCombineRows + lane, lanes = a.hkv * a.tree_blocks;
     const int mine = hk * a.tree_blocks + row / ROWS;
+    grid_wait_for_previous();
+    if (c0 == c1) return;                                    // finished by its CTA
     float m = -INFINITY, tot = 0.f;
     float4 acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float w, float t, const float4 (&v)[N]) { // a result of weight t e^w
-        if (w == -INFINITY) return;                          // a piece in which the row sees nothing
-        const float next = fmaxf(m, w), f = expf(m - next), e = expf(w - next);
-        m = next;
-        tot = tot * f + t * e;
+    // results of weights t e^w; e^w is 0 for a piece in which the row sees nothing, whose v is not used
+    auto add = [&](const float (&w)[U], const float (&t)[U], const float4 (&v)[U][N]) {
+        float next = m;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            acc[i].x = acc[i].x * f + e * v[i].x; acc[i].y = acc[i].y * f + e * v[i].y;
-            acc[i].z = acc[i].z * f + e * v[i].z; acc[i].w = acc[i].w * f + e * v[i].w;
+        for (int u = 0; u < U; ++u) next = fmaxf(next, w[u]);
+        if (next == -INFINITY) return;
+        const float f = expf(m - next);
+        m = next;
+        tot *= f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) { acc[i].x *= f; acc[i].y *= f; acc[i].z *= f; acc[i].w *= f; }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (w[u] == -INFINITY) continue;
+            const float e = expf(w[u] - next);
+            tot += t[u] * e;
+#pragma unroll
+            for (int i = 0; i < N; ++i) { acc[i].x += e * v[u][i].x; acc[i].y += e * v[u][i].y; acc[i].z += e * v[u][i].z; acc[i].w += e * v[u][i].w; }
         }
     };
     if (row < rows_all) {
-#pragma unroll 2
-        for (int c = c0 + phase; c <= c1; c += PHASES) {
-            // the piece in share c: the CTA's last one where the sequence begins in its share, else its first
-            const int64_t piece = (int64_t)(c * lanes + mine) * 2 + (c == c0 ? 1 : 0);
-            const float w = __ldcg(a.lse_part + piece * ROWS + row % ROWS);
-            float4 v[N];
+        float t[U];
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(a.o_part) + (piece * (D / 4) + cols * N + i) * ROWS + row % ROWS);
-            add(w, 1.f, v);
+        for (int u = 0; u < U; ++u) t[u] = 1.f;
+        for (int c = c0 + phase; c <= c1; c += PHASES * U) {
+            float w[U];
+            float4 v[U][N];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int cu = c + u * PHASES;
+                // the piece in share c: the CTA's last one where the sequence begins in its share, else its first
+                const int64_t piece = (int64_t)(cu * lanes + mine) * 2 + (cu == c0 ? 1 : 0);
+                w[u] = cu <= c1 ? __ldcg(a.lse_part + piece * ROWS + row % ROWS) : -INFINITY;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (cu <= c1) v[u][i] = __ldcg(reinterpret_cast<const float4*>(a.o_part) + (piece * (D / 4) + cols * N + i) * ROWS + row % ROWS);
+            }
+            add(w, t, v);
         }
     }
     if constexpr (PHASES > 1) {
-        __shared__ float s_m[PHASES][32], s_tot[PHASES][32];
-        __shared__ float4 s_acc[PHASES][N][32];
-        s_m[phase][lane] = m;
-        s_tot[phase][lane] = tot;
+        __shared__ float s_m[8][32], s_tot[8][32];
+        __shared__ float4 s_acc[8][N][32];
+        s_m[warp][lane] = m;
+        s_tot[warp][lane] = tot;
 #pragma unroll
-        for (int i = 0; i < N; ++i) s_acc[phase][i][lane] = acc[i];
+        for (int i = 0; i < N; ++i) s_acc[warp][i][lane] = acc[i];
         __syncthreads();
         if (phase) return;
-        for (int k = 1; k < PHASES; ++k) {
-            float4 v[N];
+        m = -INFINITY;
+        tot = 0.f;
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = s_acc[k][i][lane];
-            add(s_m[k][lane], s_tot[k][lane], v);
+        for (int i = 0; i < N; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < PHASES; k += U) {
+            float w[U], t[U];
+            float4 v[U][N];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int from = (k + u) * WIDE + warp;
+                const bool there = k + u < PHASES;
+                w[u] = there ? s_m[from][lane] : -INFINITY;
+                t[u] = there ? s_tot[from][lane] : 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (there) v[u][i] = s_acc[from][i][lane];
+            }
+            add(w, t, v);
         }
     }
     if (row >= rows_all) return;
@@ -671,9 +704,10 @@ int launch_t(const fa_fwd_params& p, const Sm100FwdArgs& a) {
     mark_kernel(st);
     constexpr int ROWS = DUAL ? 128 : 256;
     const int64_t blocks = (int64_t)p.b * p.hkv * ((p.sq * a.gq + kCombineRows - 1) / kCombineRows);
-    // fewer blocks than two an SM: each is made eight
-    const cudaError_t e = blocks < 2 * sm_count() ? launch_early(tree_combine_kernel<T, D, ROWS, 8>, dim3((unsigned)blocks * 8), 256, 0, st, a)
-                                                  : launch_early(tree_combine_kernel<T, D, ROWS, 1>, dim3((unsigned)blocks), 256, 0, st, a);
+    const bool many = blocks >= 2 * sm_count(), cut = a.tree_shares >= 16 * a.b;
+    const cudaError_t e = many ? launch_early(tree_combine_kernel<T, D, ROWS, D / 32, 1>, dim3((unsigned)blocks), 256, 0, st, a)
+                        : !cut ? launch_early(tree_combine_kernel<T, D, ROWS, 2, 1>, dim3((unsigned)blocks * (D / 64)), 256, 0, st, a)
+                               : launch_early(tree_combine_kernel<T, D, ROWS, 2, 8>, dim3((unsigned)blocks * (D / 8)), 256, 0, st, a);
     if (int code = cuda_ok(e, "tree_combine launch")) return code;
     mark_kernel(st);
     return FA_OK;
