@@ -1151,6 +1151,8 @@ bool fwd_sm100_tree_supported(const fa_fwd_params& p) {
     if (tree_box(p) < 8 || p.kv_entries > (1 << 24) || !(p.scale > 0.f) || p.sk <= 0) return false;
     for (const fa_tensor* t : {&p.k, &p.v})
         if (t->stride_h <= 0 || t->stride_s <= 0 || t->stride_b <= 0) return false;
+    // head dims up to 128: the shared kernel, or with a cap the one for capped scores, which caps whatever it is given
+    if (p.d <= 128 && !(p.softcap > 0.f) && !fwd_sm100_tree_shared(p)) return false;
     return encode_fn() != nullptr;
 }
 long fwd_sm100_tree_ctas(const fa_fwd_params& p) {
@@ -1163,7 +1165,8 @@ static int launch_tree_wide(const fa_fwd_params& p, Sm100FwdArgs& a) {
     if (p.d > 192) return p.softcap > 0.f ? launch_sm100_wide_b<T, 256, true, true>(p, a) : launch_sm100_wide_b<T, 256, false, true>(p, a);
     return p.softcap > 0.f ? launch_sm100_wide_b<T, 192, true, true>(p, a) : launch_sm100_wide_b<T, 192, false, true>(p, a);
 }
-// Head dims up to 128 without a cap: the kernel that shares out all key tiles evenly (tree_sm100.cu).
+// Head dims up to 128 without a cap: the kernel that shares out all key tiles evenly (tree_sm100.cu), as long as its list can be
+// counted in 32 bits whatever the lengths are; a batch whose capacities are beyond that runs on the general kernel.
 // Otherwise a CTA a split, joined by the forward's combine.
 bool fwd_sm100_tree_shared(const fa_fwd_params& p) {
     const long long tiles = ((long long)p.sk + 127) / 128 * p.b;         // at most; counted in 32 bits
@@ -1198,6 +1201,7 @@ int launch_fwd_sm100_tree(const fa_fwd_params& p, const TreeMask& tree, int nspl
         note_kernel("sm100_tcgen05_tree", dual ? FORM_SHORT_QUERIES : FORM_USUAL);
         return launch_tree_sm100(p, a, dual);
     }
+    if (p.d <= 128 && !(p.softcap > 0.f)) return fail(FA_ERR_UNSUPPORTED, "no tcgen05 kernel for this tree");
     note_kernel(p.d > 128 ? "sm100_tcgen05_wide" : "sm100_tcgen05_2q", p.d > 128 ? FORM_USUAL : FORM_ONE_TILE);
     if (p.d <= 128) return launch_fwd_single_sm100(p, a, true);
     return p.dtype == FA_F16 ? launch_tree_wide<__half>(p, a) : launch_tree_wide<__nv_bfloat16>(p, a);
