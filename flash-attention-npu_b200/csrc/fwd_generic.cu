@@ -127,6 +127,7 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
         cp_async16(smem_u32(sQ) + swz<PITCH>(r, c), src, ok ? 16 : 0);
     }
 
+    const int first_any = TREE ? tree_first_any(a.tree, L) : 0;
     auto load_kv = [&](int nb, int stage) {
         const int n0 = nb * BN;
         for (int idx = tid; idx < BN * CHUNKS; idx += 128) {
@@ -135,8 +136,9 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
             bool ok = tok < sk;
             int64_t koff = 0, voff = 0;
             if constexpr (TREE) {
-                // rows of drafted tokens that are not there hold whatever was there before; a page that is not in the cache
-                // reads as zeros, as in the tile copies
+                // rows in front of every window, and rows of drafted tokens that are not there, may hold anything, NaN included,
+                // and 0 x NaN is NaN; a page that is not in the cache reads as zeros, as in the tile copies
+                ok = ok && tok >= first_any;
                 if (ok && tok >= L) ok = (a.tree.keys[b * a.tree.words + ((tok - L) >> 5)] >> ((tok - L) & 31)) & 1;
                 if (ok) ok = (uint64_t)(int64_t)(btab ? btab[tok / p.page_size] : kb) < (uint64_t)p.kv_entries;
             }
