@@ -274,8 +274,9 @@ __global__ void __launch_bounds__(128) fwd_generic_kernel(const FwdArgs a) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const float l = quad_sum(l_i[r]);
-        inv[r] = l > 0.f ? 1.f / l : 0.f;
-        lse[r] = l > 0.f ? (m_i[r] + log2f(l)) * kLn2 : (a.part_minus_inf ? -INFINITY : INFINITY);
+        const bool none = TREE ? l == 0.f : !(l > 0.f);      // nothing seen; TREE: NaN stays NaN
+        inv[r] = none ? 0.f : 1.f / l;
+        lse[r] = none ? (a.part_minus_inf ? -INFINITY : INFINITY) : (m_i[r] + log2f(l)) * kLn2;
     }
     const bool to_part = a.o_part != nullptr;
     if (to_part) {
@@ -626,7 +627,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(
     for (int s = lane; s < nsplit; s += 32) tot += expf(w[s] - ms);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, d);
-    const float l = tot > 0.f ? ms + logf(tot) : -INFINITY;
+    const bool none = tot == 0.f || m == INFINITY;           // no split saw a key; a split whose LSE is NaN makes the row NaN
+    const float l = none ? -INFINITY : ms + logf(tot);
     // a split that saw no key (lse = -inf) gets weight 0 and its O slot is never read (it may hold anything)
     for (int s = lane; s < nsplit; s += 32) w[s] = w[s] == -INFINITY ? 0.f : expf(w[s] - l);
     __syncwarp();
@@ -678,7 +680,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(
             store_out<OutT>(o + ooff + c, acc);
         }
     }
-    if (lane == 0 && lse) lse[loff] = (tot > 0.f || keep_minus_inf) ? l : INFINITY;
+    if (lane == 0 && lse) lse[loff] = none && !keep_minus_inf ? INFINITY : l;
 }
 
 // The same for few splits: one thread per four columns of a row, all its loads (LSEs and partials) in flight at once, the
@@ -720,7 +722,8 @@ __global__ void __launch_bounds__(256) combine_few_kernel(
         for (int s = 0; s < d; ++s) e[s] += e[s + d];
     }
     const float tot = e[0];
-    const float l = tot > 0.f ? ms + logf(tot) : -INFINITY;
+    const bool none = tot == 0.f || m == INFINITY;           // as above
+    const float l = none ? -INFINITY : ms + logf(tot);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -744,7 +747,7 @@ __global__ void __launch_bounds__(256) combine_few_kernel(
     typename Out4<OutT>::V pk;
     memcpy(&pk, out, sizeof(pk));
     *reinterpret_cast<typename Out4<OutT>::V*>(o + ooff + c) = pk;
-    if (c == 0 && lse) lse[loff] = (tot > 0.f || keep_minus_inf) ? l : INFINITY;
+    if (c == 0 && lse) lse[loff] = none && !keep_minus_inf ? INFINITY : l;
 }
 
 // 16-byte reads of the partials and four outputs a store; several warps may share a row, so the LSEs are not written

@@ -484,7 +484,8 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
         if (ok) ok = mbar_wait(bar(N_O), 0, abort_flag, err, 90);
         if (ok) {
             tc_fence_after();
-            const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
+            const bool none = TREE ? l_tot == 0.f : !(l_tot > 0.f);      // nothing seen; TREE: NaN stays NaN
+            const float inv = none ? 0.f : 1.f / l_tot;
             T* orow = out_row(r) + half * (D / 2);
             float* prow = a.nsplit > 1 ? a.o_part + part_row(r) * a.d + half * (D / 2) : nullptr;
             const int left = a.d - half * (D / 2);           // columns of the call's head dim from here on
@@ -517,8 +518,8 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
                     }
                 }
             }
-            if (half == 0 && r < rows && prow) a.lse_part[part_row(r)] = l_tot > 0.f ? (m_used + log2f(l_tot)) * kLn2 : -INFINITY;
-            else if (half == 0 && r < rows && a.lse) *lse_slot(r) = l_tot > 0.f ? (m_used + log2f(l_tot)) * kLn2 : INFINITY;
+            if (half == 0 && r < rows && prow) a.lse_part[part_row(r)] = none ? -INFINITY : (m_used + log2f(l_tot)) * kLn2;
+            else if (half == 0 && r < rows && a.lse) *lse_slot(r) = none ? INFINITY : (m_used + log2f(l_tot)) * kLn2;
         }
     }
     tc_fence_before();

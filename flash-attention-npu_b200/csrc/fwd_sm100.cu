@@ -837,6 +837,8 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
         const float cap_out = a.softcap * kLog2e;
         const float slope = (BIAS && a.alibi) ? a.alibi[(int64_t)b * a.alibi_sb + h] * kLog2e : 0.f;
         const float rel = (float)(qi + sk - sq);
+        // TREE: NaN when a score is, which the polynomial exponential loses
+        auto max3 = [](float x, float y, float z) { return TREE ? max3_nan(x, y, z) : fmaxf(fmaxf(x, y), z); };
         bool ok = true;
         for (int j = 0; j < ntiles && ok; ++j) {
             const int n0 = (t_lo + j) * 128, buf = j & 1;
@@ -888,14 +890,14 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
                 for (int c = 2 * hh; c < 2 * hh + 2; ++c) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
-                        mx0 = fmaxf(fmaxf(mx0, __uint_as_float(sreg[c][i])), __uint_as_float(sreg[c][i + 1]));
-                        mx1 = fmaxf(fmaxf(mx1, __uint_as_float(sreg[c][i + 2])), __uint_as_float(sreg[c][i + 3]));
-                        mx2 = fmaxf(fmaxf(mx2, __uint_as_float(sreg[c][i + 4])), __uint_as_float(sreg[c][i + 5]));
-                        mx3 = fmaxf(fmaxf(mx3, __uint_as_float(sreg[c][i + 6])), __uint_as_float(sreg[c][i + 7]));
+                        mx0 = max3(mx0, __uint_as_float(sreg[c][i]), __uint_as_float(sreg[c][i + 1]));
+                        mx1 = max3(mx1, __uint_as_float(sreg[c][i + 2]), __uint_as_float(sreg[c][i + 3]));
+                        mx2 = max3(mx2, __uint_as_float(sreg[c][i + 4]), __uint_as_float(sreg[c][i + 5]));
+                        mx3 = max3(mx3, __uint_as_float(sreg[c][i + 6]), __uint_as_float(sreg[c][i + 7]));
                     }
                 }
             }
-            const float m_new = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sc;       // log2 domain
+            const float m_new = max3(max3(mx0, mx1, mx2), mx3, mx3) * sc;       // log2 domain
             if (m_used == -INFINITY) m_used = m_new;
             if (j > 0 && __any_sync(0xffffffffu, m_new > m_used + kRescaleThreshold)) {
                 // P V of tile j - 1 was issued AFTER the scores of this tile: wait for it before touching O
@@ -946,12 +948,14 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
             if (full) exp_phase(std::integral_constant<int, kFwdPoly<D>>{});
             else exp_phase(std::integral_constant<int, 0>{});
             l_run += (sum_a.x + sum_b.x) + (sum_a.y + sum_b.y);
+            if (TREE && m_new != m_new) l_run = m_new;
         }
         if (ok) ok = mbar_wait(bar(W_O), 0, abort_flag, err, 10);
         if (TREE && !there) l_run = 0.f;
         if (ok) {
             tc_fence_after();
-            const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+            const bool none = TREE ? l_run == 0.f : !(l_run > 0.f);      // nothing seen; TREE: NaN stays NaN
+            const float inv = none ? 0.f : 1.f / l_run;
             T* orow = out_row(r);
             float* prow = TREE && a.nsplit > 1 ? a.o_part + part_row(r) * a.d : nullptr;
 #pragma unroll 1
@@ -983,8 +987,8 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
                     }
                 }
             }
-            if (TREE && r < rows && prow) a.lse_part[part_row(r)] = l_run > 0.f ? (m_used + log2f(l_run)) * kLn2 : -INFINITY;
-            else if (r < rows && a.lse) *lse_slot(r) = l_run > 0.f ? (m_used + log2f(l_run)) * kLn2 : INFINITY;
+            if (TREE && r < rows && prow) a.lse_part[part_row(r)] = none ? -INFINITY : (m_used + log2f(l_run)) * kLn2;
+            else if (r < rows && a.lse) *lse_slot(r) = none ? INFINITY : (m_used + log2f(l_run)) * kLn2;
         }
     }
     }

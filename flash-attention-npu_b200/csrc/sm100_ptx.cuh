@@ -85,6 +85,18 @@ __device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity,
     return true;
 }
 
+// ---- maxima that are NaN when one of the values is ------------------------------------------------------------
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // ---- programmatic dependent launch -------------------------------------------------------------------------
 // A grid launched with the attribute may start once every CTA of the grid in front has called grid_let_next_start() or left;
 // grid_wait_for_previous() waits until that grid has completed and its writes are visible.  (Without the attribute both do

@@ -437,19 +437,19 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
                             if (!(vis >> i & 1)) sreg[c][i] = 0xff800000u;     // -inf
                     }
                 }
-                // four independent chains of three-input maxima
+                // four independent chains of three-input maxima, NaN when a visible score is: the polynomial exponential loses it
 #pragma unroll
                 for (int c = 2 * hh; c < 2 * hh + 2; ++c) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 8) {
-                        mx0 = fmaxf(fmaxf(mx0, __uint_as_float(sreg[c][i])), __uint_as_float(sreg[c][i + 1]));
-                        mx1 = fmaxf(fmaxf(mx1, __uint_as_float(sreg[c][i + 2])), __uint_as_float(sreg[c][i + 3]));
-                        mx2 = fmaxf(fmaxf(mx2, __uint_as_float(sreg[c][i + 4])), __uint_as_float(sreg[c][i + 5]));
-                        mx3 = fmaxf(fmaxf(mx3, __uint_as_float(sreg[c][i + 6])), __uint_as_float(sreg[c][i + 7]));
+                        mx0 = max3_nan(mx0, __uint_as_float(sreg[c][i]), __uint_as_float(sreg[c][i + 1]));
+                        mx1 = max3_nan(mx1, __uint_as_float(sreg[c][i + 2]), __uint_as_float(sreg[c][i + 3]));
+                        mx2 = max3_nan(mx2, __uint_as_float(sreg[c][i + 4]), __uint_as_float(sreg[c][i + 5]));
+                        mx3 = max3_nan(mx3, __uint_as_float(sreg[c][i + 6]), __uint_as_float(sreg[c][i + 7]));
                     }
                 }
             }
-            const float m_new = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sc;       // log2 domain
+            const float m_new = max_nan(max3_nan(mx0, mx1, mx2), mx3) * sc;       // log2 domain
             if (m_used == -INFINITY) m_used = m_new;
             if (j > 0 && __any_sync(0xffffffffu, m_new > m_used + kRescaleThreshold)) {
                 const float m_next = fmaxf(m_used, m_new);
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
             };
             if (full) exp_phase(std::integral_constant<int, D == 128 ? 1 : 2>{});
             else exp_phase(std::integral_constant<int, 0>{});
-            l_run += (sum_a.x + sum_b.x) + (sum_a.y + sum_b.y);
+            l_run = m_new != m_new ? m_new : l_run + ((sum_a.x + sum_b.x) + (sum_a.y + sum_b.y));
         }
         // ---- end of the piece ----
         float f_a = 1.f, f_b = 0.f;                          // DUAL: weights of the two groups' results
@@ -522,7 +522,8 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
         tc_fence_after();
         const bool there = first_key() != 0x7fffffff;
         if (!there) l_run = 0.f;                             // no token: whatever its q holds, zeros and no LSE
-        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+        // a row sum of 0 says that nothing was seen; NaN stays NaN
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         T* orow = reinterpret_cast<T*>(a.o) + (int64_t)p.b * a.o_sb + (int64_t)qi * a.o_ss + (int64_t)head * a.o_sh;
         // partials: four columns of all rows, then the next four, so that a warp's stores lie side by side
         const int64_t piece = (int64_t)blockIdx.x * 2 + (p.head ? 1 : 0);
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
         tc_fence_before();
         mbar_arrive(bar(DUAL ? (int)R_OE0 : R_OE0 + x));
         if (mine && !(DUAL && x)) {
-            const float lse = l_run > 0.f ? (m_used + log2f(l_run)) * kLn2 : p.whole ? INFINITY : -INFINITY;
+            const float lse = l_run != 0.f ? (m_used + log2f(l_run)) * kLn2 : p.whole ? INFINITY : -INFINITY;
             if (!p.whole) a.lse_part[piece * ROWS + x0 + r] = lse;
             else if (a.lse) a.lse[(int64_t)p.b * a.lse_sb + (int64_t)head * a.lse_sh + (int64_t)qi * a.lse_ss] = lse;
         }
@@ -612,11 +613,12 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
     float4 acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    // results of weights t e^w; e^w is 0 for a piece in which the row sees nothing, whose v is not used
+    // results of weights t e^w; e^w is 0 for a piece in which the row sees nothing, whose v is not used.  A piece of a row that
+    // holds NaN has a NaN w, and makes m, the sum and the output NaN.
     auto add = [&](const float (&w)[U], const float (&t)[U], const float4 (&v)[U][N]) {
         float next = m;
 #pragma unroll
-        for (int u = 0; u < U; ++u) next = fmaxf(next, w[u]);
+        for (int u = 0; u < U; ++u) next = max_nan(next, w[u]);
         if (next == -INFINITY) return;
         const float f = expf(m - next);
         m = next;
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
         }
     }
     if (row >= rows_all) return;
-    const float inv = tot > 0.f ? 1.f / tot : 0.f;
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;
     const int qi = row / a.gq, head = hk * a.gq + row % a.gq;
     T* orow = reinterpret_cast<T*>(a.o) + (int64_t)b * a.o_sb + (int64_t)qi * a.o_ss + (int64_t)head * a.o_sh + cols * N * 4;
 #pragma unroll
@@ -691,7 +693,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const __grid_constant
             reinterpret_cast<uint4*>(orow)[i / 2] = make_uint4(Elem<T>::pack(acc[i].x * inv, acc[i].y * inv), Elem<T>::pack(acc[i].z * inv, acc[i].w * inv),
                                                                Elem<T>::pack(acc[i + 1].x * inv, acc[i + 1].y * inv), Elem<T>::pack(acc[i + 1].z * inv, acc[i + 1].w * inv));
     if (cols == 0 && a.lse)
-        a.lse[(int64_t)b * a.lse_sb + (int64_t)head * a.lse_sh + (int64_t)qi * a.lse_ss] = tot > 0.f ? m + logf(tot) : INFINITY;
+        a.lse[(int64_t)b * a.lse_sb + (int64_t)head * a.lse_sh + (int64_t)qi * a.lse_ss] = tot == 0.f ? INFINITY : m + logf(tot);
 }
 
 template <typename T, int D, bool DUAL>
