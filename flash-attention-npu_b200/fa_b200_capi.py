@@ -348,6 +348,32 @@ def plain(*tensors):
     return True
 
 
+def _transform_state():
+    """-> a function that says whether a functorch transform or a forward-mode level is active; always yes, as above, where
+    torch lacks a name."""
+    try:
+        functorch, forward_ad = torch._C._functorch.peek_interpreter_stack, torch.autograd.forward_ad
+
+        def active():
+            return functorch() is not None or forward_ad._current_level >= 0
+
+        active()
+        return active
+    except AttributeError:
+        return lambda: True
+
+
+transforming = _transform_state()
+
+
+def has_tangent(t):
+    """True for a dual tensor, or one that a functorch transform follows: what is written into its memory reaches neither."""
+    if not transforming():
+        return False
+    wrapped = getattr(getattr(torch._C, "_functorch", None), "is_functorch_wrapped_tensor", None)
+    return wrapped is None or wrapped(t) or torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 

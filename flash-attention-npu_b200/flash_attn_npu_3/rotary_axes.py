@@ -118,45 +118,80 @@ def _rotary_axes_fake(q, k, cos, sin, positions, sections, cyclic, interleaved, 
     return q.new_empty(q.shape), q.new_empty((0,)) if k is None else k.new_empty(k.shape)
 
 
-def _forward(q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
-    if capi.plain(q, k, cos, sin):                             # the op's dispatch would do nothing but call the body
-        return _out_of_place(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
-    q_out, k_out = _rotary_axes(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
+def _by_op(q, k, *args):
+    q_out, k_out = _rotary_axes(q, k, *args)
     return q_out, None if k is None else k_out
+
+
+def _forward(q, k, cos, sin, *args):
+    if capi.plain(q, k, cos, sin):                             # the op's dispatch would do nothing but call the body
+        return _out_of_place(q, k, cos, sin, *args)
+    return _by_op(q, k, cos, sin, *args)
+
+
+def _turn_two(turn, q, k, *args):
+    """turn(q, k, *args) for gradients or tangents, each of which may be missing."""
+    if q is not None:
+        return turn(q, k, *args)
+    return (None, None) if k is None else (None, turn(k, None, *args)[0])
 
 
 class RotaryAxesFunc(torch.autograd.Function):
     """A rotation is linear and orthogonal: its gradient is the rotation back, which is differentiable in the same way."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
+    def forward(ctx, *inputs):
         ctx.set_materialize_grads(False)
+        RotaryAxesFunc.keep(ctx, inputs)
+        return _forward(*inputs)
+
+    @staticmethod
+    def keep(ctx, inputs):
+        _, _, cos, sin, positions, sections, cyclic, interleaved, backward = inputs
         ctx.save_for_backward(cos, sin, positions)
         ctx.args = (sections, cyclic, interleaved)
         ctx.turn_back = not backward
-        return _forward(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        cos, sin, positions = ctx.saved_tensors
-        args = (cos, sin, positions, *ctx.args, ctx.turn_back)
-        if dq is not None and dk is not None:
-            dq, dk = _apply(dq, dk, *args)
-        elif dq is not None:
-            dq, _ = _apply(dq, None, *args)
-        elif dk is not None:
-            dk, _ = _apply(dk, None, *args)
-        return (dq, dk) + (None,) * 7
+        return _turn_two(_apply, dq, dk, *ctx.saved_tensors, *ctx.args, ctx.turn_back) + (None,) * 7
+
+
+class RotaryAxesTransformFunc(torch.autograd.Function):
+    """The same where a functorch transform or a forward-mode level is active (torch takes 26 us longer to call this kind): the
+    derivative in a direction is the rotation of the direction.  Always by the op: what a transform has saved is still wrapped
+    when a gradient is asked for after its end.  Missing directions come as zeros: torch takes no None for a tensor's tangent."""
+    generate_vmap_rule = True
+
+    @staticmethod
+    def forward(q, k, cos, sin, positions, sections, cyclic, interleaved, backward):
+        return _by_op(q, k, cos, sin, positions, sections, cyclic, interleaved, backward)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        RotaryAxesFunc.keep(ctx, inputs)
+        ctx.save_for_forward(*inputs[2:5])
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        return _turn_two(RotaryAxesTransformFunc.apply, dq, dk, *ctx.saved_tensors, *ctx.args, ctx.turn_back) + (None,) * 7
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        return _turn_two(RotaryAxesTransformFunc.apply, tq, tk, *ctx.saved_tensors, *ctx.args, not ctx.turn_back)
 
 
 def _apply(q, k, *args):
+    if capi.transforming():
+        return RotaryAxesTransformFunc.apply(q, k, *args)
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return RotaryAxesFunc.apply(q, k, *args)
     return _forward(q, k, *args)
 
 
 def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=False, interleaved=False, inplace=False):
-    """Rotary embedding of q and k with one to four position axes (time, height, width, ..), differentiable in q and k.
+    """Rotary embedding of q and k with one to four position axes (time, height, width, ..), differentiable in q and k (in
+    reverse and forward mode).
 
     q (batch, seqlen, nheads, headdim) or packed (total, nheads, headdim), fp16 or bf16; k of the same shape but for its heads,
     or None.  cos / sin (seqlen_ro, rotary_dim / 2) in q's dtype or fp32.  positions int32 (axes, batch, seqlen) or
@@ -203,6 +238,8 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
                 continue
             if torch.is_grad_enabled() and t.requires_grad:
                 raise RuntimeError("inplace rotary embedding is not differentiable: detach q and k, or leave inplace out")
+            if capi.has_tangent(t):
+                raise RuntimeError("inplace rotary embedding has no forward-mode derivatives and no function transforms: leave inplace out")
             if t.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise RuntimeError("inplace rotary embedding needs a contiguous last dimension and no expanded dimensions")
         if k is not None and k.data_ptr() == q.data_ptr() and k.numel():
