@@ -168,12 +168,12 @@ def mla_decode(q_nope, q_rope, latent_i8, scales, rope, block_table, cache_seqle
 
 
 def _input(t):
-    """An input and the four leaves of its fa_tensor, as 16-byte loads can read it: a copy where its last dim is strided or its
-    rows are not aligned."""
+    """An input and the four leaves of its fa_tensor, as 16-byte loads can read it: a copy where its last dim is strided, its rows
+    are not aligned, or it is lazily negated."""
     s0, s1, s2, s3 = t.stride()
     ptr = t.data_ptr()
-    if s3 != 1 or ptr & 15 or (s0 | s1 | s2) & 7:
-        t = t.clone(memory_format=torch.contiguous_format)
+    if s3 != 1 or ptr & 15 or (s0 | s1 | s2) & 7 or t.is_neg():
+        t = t.resolve_neg().clone(memory_format=torch.contiguous_format)
         s0, s1, s2, s3 = t.stride()
         ptr = t.data_ptr()
     return t, (ptr, s0, s1, s2)
@@ -217,6 +217,8 @@ def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cac
     kc, vc = k_cache.stride(), v_cache.stride()
     if kc[3] != 1 or vc[3] != 1:
         raise RuntimeError("k_cache and v_cache must have contiguous last dimension")
+    if k_cache.is_neg() or v_cache.is_neg():
+        raise RuntimeError("k_cache and v_cache may not be lazily negated")
     if (k is None) != (v is None):
         raise RuntimeError("k and v must be passed together")
     if window_size_right != -1 and window_size_right != 0:
@@ -277,10 +279,10 @@ def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cac
         rows_ro, pairs = shape
         if rows_ro == 0 or not 0 < 2 * pairs <= d:
             raise RuntimeError("rotary_dim must be positive and at most the head dimension, with one table row at least")
-        if rotary_cos.dtype is not dtype or not rotary_cos.is_contiguous():
-            rotary_cos = rotary_cos.to(dtype).contiguous()
-        if rotary_sin.dtype is not dtype or not rotary_sin.is_contiguous():
-            rotary_sin = rotary_sin.to(dtype).contiguous()
+        if rotary_cos.dtype is not dtype or not rotary_cos.is_contiguous() or rotary_cos.is_neg():
+            rotary_cos = rotary_cos.to(dtype).resolve_neg().contiguous()
+        if rotary_sin.dtype is not dtype or not rotary_sin.is_contiguous() or rotary_sin.is_neg():
+            rotary_sin = rotary_sin.to(dtype).resolve_neg().contiguous()
         rotary = (rotary_cos.data_ptr(), rotary_sin.data_ptr(), 2 * pairs, 1 if rotary_interleaved else 0, rows_ro)
         if rotary_sections is not None:
             keep, where, n = axis_pointer(pairs, rotary_sections, rotary_sections_cyclic)

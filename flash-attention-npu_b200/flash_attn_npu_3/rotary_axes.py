@@ -201,6 +201,9 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
     i belongs to axis i % axes while that axis has pairs left, else to axis 0.  None: one axis.  A position outside the tables
     takes the nearest row.  fp32 arithmetic, rounded once; cos, sin and positions get no gradient.
 
+    (Dual tensors given to a function that torch.compile has traced lose their tangent, as in every custom op; torch.func.jvp
+    inside or around it does not.)
+
     inplace writes into q and k instead of new tensors (only where no gradient is needed); q and k must not share memory.
     Returns (q, k), or q alone when k is None."""
     index, dtype, shape = capi.cuda_index(q), q.dtype, q.shape
@@ -244,7 +247,9 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
                 raise RuntimeError("inplace rotary embedding needs a contiguous last dimension and no expanded dimensions")
         if k is not None and k.data_ptr() == q.data_ptr() and k.numel():
             raise RuntimeError("inplace rotary embedding needs q and k in memory of their own")
-        _run(q, k, *args, False, True)
+        # the op's dispatch reads lazily negated tables with their sign; here nothing stands in front of the kernel.  (q and k may
+        # be such views: what is turned is the memory, and the turned negative is the negative of the turned.)
+        _run(q, k, cos.resolve_neg(), sin.resolve_neg(), *args[2:], False, True)
         torch.autograd.graph.increment_version(q if k is None else (q, k))
     else:
         q, k = _apply(q, k, *args, False)
