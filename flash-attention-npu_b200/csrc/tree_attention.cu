@@ -37,7 +37,8 @@ struct TreePrepArgs {
 // token knows its 2^k nearest ancestors, so eight rounds do for any tree of 256 tokens.  (Climbing one parent a step took 18 us
 // for a chain of 64 tokens.)
 constexpr int kPrepItems = 1;
-template <typename T, bool VEC>
+// TT: the tables' type, T or float
+template <typename T, typename TT, bool VEC>
 __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_constant__ TreePrepArgs a) {
     // what a token has climbed to: the token there, or -1 = the cached rows, -2 = no token; and over how many
     __shared__ short s_up[2][kTreeMaxTokens], s_depth[2][kTreeMaxTokens], s_parent[kTreeMaxTokens];
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
             int lo, hi;
             unit_chunks(a.ro, u, lo, hi);
             float c[8], s[8];
-            load_angles<T>(a.ro, rows, u * 8, c, s);
+            load_angles<TT>(a.ro, rows, u * 8, c, s);
             uint4 ya, yb;
             turn_chunks<T>(s4[lo], s4[hi], c, s, a.ro.interleaved, ya, yb);
             d4[lo] = ya;
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
             d4[2 * u] = x;
         }
     } else {
-        for (int e = u * 16; e < min(n, u * 16 + 16); ++e) dst[e] = rd ? turn_elem<T, T>(src, e, a.ro, rows, 1.f) : src[e];
+        for (int e = u * 16; e < min(n, u * 16 + 16); ++e) dst[e] = rd ? turn_elem<T, TT>(src, e, a.ro, rows, 1.f) : src[e];
     }
     }
 }
@@ -226,6 +227,12 @@ void plan_tree(const fa_fwd_params& p, TreePlan& plan) {
 bool tree_vec_ok(const fa_fwd_params& p) {
     if (!p.rotary_cos) return true;
     return p.rotary_dim % 16 == 0 && ((reinterpret_cast<uintptr_t>(p.rotary_cos) | reinterpret_cast<uintptr_t>(p.rotary_sin)) & 15) == 0;
+}
+
+template <typename T, typename TT>
+void launch_prep(const TreePrepArgs& a, dim3 grid, cudaStream_t st) {
+    if (tree_vec_ok(a.p)) tree_prep_kernel<T, TT, true><<<grid, kTreeMaxTokens, 0, st>>>(a);
+    else tree_prep_kernel<T, TT, false><<<grid, kTreeMaxTokens, 0, st>>>(a);
 }
 
 int check_tensor(const char* name, const fa_tensor& t) {
@@ -313,14 +320,9 @@ int run_tree(const fa_tree_params& t) {
     a.items_kv = a.items_k + (p.k_new.ptr ? p.sq * p.hkv * a.uv : 0);
     a.items = a.items_kv + p.sq * p.hq * a.uk;
     const dim3 grid((a.items + kPrepItems * kTreeMaxTokens - 1) / (kPrepItems * kTreeMaxTokens), p.b);
-    const bool vec = tree_vec_ok(p);
-    if (p.dtype == FA_F16) {
-        if (vec) tree_prep_kernel<__half, true><<<grid, kTreeMaxTokens, 0, st>>>(a);
-        else tree_prep_kernel<__half, false><<<grid, kTreeMaxTokens, 0, st>>>(a);
-    } else {
-        if (vec) tree_prep_kernel<__nv_bfloat16, true><<<grid, kTreeMaxTokens, 0, st>>>(a);
-        else tree_prep_kernel<__nv_bfloat16, false><<<grid, kTreeMaxTokens, 0, st>>>(a);
-    }
+    const bool fp32 = p.rotary_cos && t.tables_fp32;
+    if (p.dtype == FA_F16) fp32 ? launch_prep<__half, float>(a, grid, st) : launch_prep<__half, __half>(a, grid, st);
+    else fp32 ? launch_prep<__nv_bfloat16, float>(a, grid, st) : launch_prep<__nv_bfloat16, __nv_bfloat16>(a, grid, st);
     mark_kernel(st);
     if (int e = cuda_ok(cudaGetLastError(), "tree_prep launch")) return e;
 

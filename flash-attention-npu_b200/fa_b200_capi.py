@@ -42,7 +42,7 @@ class TreeParams(C.Structure):
     _fields_ = [
         ("fwd", FwdParams), ("parents", C.c_void_p), ("parents_stride_b", C.c_int64),
         ("positions", C.c_void_p), ("positions_stride_axis", C.c_int64), ("positions_stride_b", C.c_int64),
-        ("axis_of_pair", C.c_void_p), ("axes", C.c_int32),
+        ("axis_of_pair", C.c_void_p), ("axes", C.c_int32), ("tables_fp32", C.c_int32),
     ]
 
 

@@ -262,7 +262,7 @@ def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cac
             raise RuntimeError("the cache has fewer entries than the batch")
     if capacity >= 2 ** 31:
         raise RuntimeError("a sequence of the cache has at most 2^31 - 1 rows")
-    rotary, positions, axes = (0, 0, 0, 0, 0), (0, 0, 0), (0, 1)
+    rotary, positions, axes, fp32 = (0, 0, 0, 0, 0), (0, 0, 0), (0, 1), 0
     keep = None
     if rotary_cos is None:
         if rotary_positions is not None or rotary_sections is not None:
@@ -279,10 +279,13 @@ def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cac
         rows_ro, pairs = shape
         if rows_ro == 0 or not 0 < 2 * pairs <= d:
             raise RuntimeError("rotary_dim must be positive and at most the head dimension, with one table row at least")
-        if rotary_cos.dtype is not dtype or not rotary_cos.is_contiguous() or rotary_cos.is_neg():
-            rotary_cos = rotary_cos.to(dtype).resolve_neg().contiguous()
-        if rotary_sin.dtype is not dtype or not rotary_sin.is_contiguous() or rotary_sin.is_neg():
-            rotary_sin = rotary_sin.to(dtype).resolve_neg().contiguous()
+        kind = dtype
+        if rotary_cos.dtype is torch.float32 and rotary_sin.dtype is torch.float32:
+            kind, fp32 = torch.float32, 1
+        if rotary_cos.dtype is not kind or not rotary_cos.is_contiguous() or rotary_cos.is_neg():
+            rotary_cos = rotary_cos.to(kind).resolve_neg().contiguous()
+        if rotary_sin.dtype is not kind or not rotary_sin.is_contiguous() or rotary_sin.is_neg():
+            rotary_sin = rotary_sin.to(kind).resolve_neg().contiguous()
         rotary = (rotary_cos.data_ptr(), rotary_sin.data_ptr(), 2 * pairs, 1 if rotary_interleaved else 0, rows_ro)
         if rotary_sections is not None:
             keep, where, n = axis_pointer(pairs, rotary_sections, rotary_sections_cyclic)
@@ -310,7 +313,7 @@ def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cac
         0, 0, cache_seqlens.data_ptr(), *table, batch_idx, 0, 0,
         batch, tokens, capacity, 0, 0, hq, hkv, d, d, softmax_scale, softcap, 0, _v2._i32(window_size_left), -1, code,
         *new, tokens, *rotary, num_splits, 0, 0, 0, 0, 0, 0, 0, 0, entries, capi.raw_stream_of(index),
-        tree_parents.data_ptr(), parents_sb, *positions, *axes)
+        tree_parents.data_ptr(), parents_sb, *positions, *axes, fp32)
     nbytes = capi._tree_bytes(buf)
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     capi.set_workspace(capi.TREE_BLOCK, buf, ws, nbytes, "fwd.")

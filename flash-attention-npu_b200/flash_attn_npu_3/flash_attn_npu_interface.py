@@ -390,9 +390,9 @@ def flash_attn_tree_with_kvcache(q, k_cache, v_cache, k, v, tree_parents,
     K that it sees, makes its output and its softmax_lse NaN.
 
     Position of a token: cache_seqlens + its depth.  window_size = (left, -1) keeps keys at most `left` positions back.
-    rotary_cos / rotary_sin (seqlen_ro, rotary_dim / 2), taken in q's dtype, turn q and k by the row of that position, or by
-    rotary_positions (axes, batch, tokens) int32 with rotary_sections = pairs of each axis (see rotary_axes_func).  A position
-    outside the tables takes the nearest row.  Rows past the cache's capacity, or on a page that is not in the cache, are
+    rotary_cos / rotary_sin (seqlen_ro, rotary_dim / 2), both fp32 or else taken in q's dtype, turn q and k by the row of that
+    position, or by rotary_positions (axes, batch, tokens) int32 with rotary_sections = pairs of each axis (see
+    rotary_axes_func, which gives the same bits).  A position outside the tables takes the nearest row.  Rows past the cache's capacity, or on a page that is not in the cache, are
     neither written nor seen.  num_splits: 0 splits the keys so that the GPU is filled, n > 0 into at most about n parts a
     sequence; the result depends on it by rounding alone.  Returns out (batch, tokens, nheads, headdim), or (out, softmax_lse (batch, nheads, tokens))."""
     if softmax_scale is None:

@@ -158,6 +158,7 @@ typedef struct {
     int64_t        positions_stride_axis, positions_stride_b;
     const uint8_t* axis_of_pair;          /* HOST, rotary_dim / 2 bytes, or null = axis 0     */
     int32_t        axes;                  /* 1 .. 4                                          */
+    int32_t        tables_fp32;           /* 0: fwd.rotary_cos / rotary_sin are of q's dtype; else fp32 */
 } fa_tree_params;
 
 int    fa_tree_fwd_kvcache(const fa_tree_params* p);
