@@ -356,7 +356,8 @@ int fa_tree_fwd_kvcache(const fa_tree_params* t) {
 }
 
 size_t fa_tree_workspace_bytes(const fa_tree_params* t) {
-    if (!t || t->fwd.b <= 0 || t->fwd.sq <= 0 || t->fwd.hq <= 0 || t->fwd.hkv <= 0 || t->fwd.d <= 0 || t->fwd.sk < 0) return 0;
+    if (!t || t->fwd.b <= 0 || t->fwd.sq <= 0 || t->fwd.hq <= 0 || t->fwd.hkv <= 0 || t->fwd.d <= 0 || t->fwd.sk < 0 ||
+        t->fwd.hq % t->fwd.hkv) return 0;
     TreePlan plan;
     plan_tree(t->fwd, plan);
     return plan.total;
