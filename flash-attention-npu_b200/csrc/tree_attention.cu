@@ -160,6 +160,8 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
     }
 }
 
+constexpr long kMaxGridY = 65535;
+
 struct TreePlan {
     int nsplit, min_keys, words, sm100, shared, shares;
     size_t bits, depth, keys, q, o, lse, total;
@@ -203,7 +205,8 @@ void plan_tree(const fa_fwd_params& p, TreePlan& plan) {
     long n = p.num_splits > 0 ? p.num_splits : plan.sm100 && base * (resident + 1) <= slots ? slots / base : (waves * slots + base - 1) / base;
     if (n > most) n = most;
     if (n > 256) n = 256;
-    if (n > 65535 / p.b) n = 65535 / p.b;
+    if (n > 65535 / p.b) n = 65535 / p.b;                    // the general kernel's grid, and
+    if (plan.sm100 && n > kMaxGridY / ((rows + 127) / 128)) n = kMaxGridY / ((rows + 127) / 128);       // the tcgen05 kernels': row blocks x splits
     plan.nsplit = (int)(n < 1 ? 1 : n);
     const size_t toks = (size_t)p.b * p.sq;
     plan.bits = 0;
@@ -249,6 +252,8 @@ int check_tree(const fa_tree_params& t) {
     if (p.b < 0 || p.sq < 0 || p.sk < 0 || p.hq <= 0 || p.hkv <= 0) return fail(FA_ERR_BAD_SHAPE, "negative or zero size");
     if (p.hq % p.hkv) return fail(FA_ERR_BAD_SHAPE, "number of heads in q must be divisible by the number of heads in k/v");
     if (p.hkv > 65535 || p.b > 65535) return fail(FA_ERR_BAD_SHAPE, "at most 65535 sequences and KV heads");
+    if ((int64_t)p.sq * (p.hq / p.hkv) > kMaxGridY * 128 || (int64_t)p.sq * (p.hq + 2ll * p.hkv) * 16 >= (1ll << 31))
+        return fail(FA_ERR_BAD_SHAPE, "at most 2^27 heads of tokens a sequence, 8388480 of them a KV head");
     if (p.d <= 0 || p.d > 256 || p.d != p.dv || p.d % 8) return fail(FA_ERR_BAD_SHAPE, "head dimension must be a multiple of 8 in [8, 256], the same for q, k and v");
     if (p.sq > kTreeMaxTokens) return fail(FA_ERR_UNSUPPORTED, "at most %d drafted tokens a sequence", kTreeMaxTokens);
     if (p.cu_seqlens_q || p.cu_seqlens_k) return fail(FA_ERR_UNSUPPORTED, "drafted tokens are not packed");
