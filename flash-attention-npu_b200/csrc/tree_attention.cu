@@ -251,6 +251,7 @@ int check_tree(const fa_tree_params& t) {
     if (p.dtype != FA_F16 && p.dtype != FA_BF16) return fail(FA_ERR_BAD_DTYPE, "only fp16 and bf16 are supported");
     if (p.b < 0 || p.sq < 0 || p.sk < 0 || p.hq <= 0 || p.hkv <= 0) return fail(FA_ERR_BAD_SHAPE, "negative or zero size");
     if (p.hq % p.hkv) return fail(FA_ERR_BAD_SHAPE, "number of heads in q must be divisible by the number of heads in k/v");
+    if (p.sk > kTreeMaxRows) return fail(FA_ERR_BAD_SHAPE, "a sequence of the cache has at most 2^31 - 1024 rows");
     if (p.hkv > 65535 || p.b > 65535) return fail(FA_ERR_BAD_SHAPE, "at most 65535 sequences and KV heads");
     if ((int64_t)p.sq * (p.hq / p.hkv) > kMaxGridY * 128 || (int64_t)p.sq * (p.hq + 2ll * p.hkv) * 16 >= (1ll << 31))
         return fail(FA_ERR_BAD_SHAPE, "at most 2^27 heads of tokens a sequence, 8388480 of them a KV head");

@@ -11,6 +11,8 @@ namespace fa {
 
 constexpr int kTreeMaxTokens = 256;
 constexpr int kTreeMaxWords = kTreeMaxTokens / 32;
+// Capacity of a sequence: rows are counted in 32 bits, up to 256 tokens and the rest of a tile behind the last one
+constexpr int kTreeMaxRows = 0x7fffffff - 1023;
 
 struct TreeMask {
     const uint32_t* bits;        // (b, tokens, words): drafted tokens that a token sees

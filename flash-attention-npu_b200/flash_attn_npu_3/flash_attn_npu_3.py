@@ -260,8 +260,8 @@ def tree_fwd_kvcache(q, k_cache, v_cache, k, v, tree_parents, cache_seqlens, cac
             batch_idx = cache_batch_idx.data_ptr()
         elif entries < batch:
             raise RuntimeError("the cache has fewer entries than the batch")
-    if capacity >= 2 ** 31:
-        raise RuntimeError("a sequence of the cache has at most 2^31 - 1 rows")
+    if capacity > 2 ** 31 - 1024:
+        raise RuntimeError("a sequence of the cache has at most 2^31 - 1024 rows")
     rotary, positions, axes, fp32 = (0, 0, 0, 0, 0), (0, 0, 0), (0, 1), 0
     keep = None
     if rotary_cos is None:

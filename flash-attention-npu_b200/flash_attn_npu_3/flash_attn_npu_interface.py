@@ -392,9 +392,10 @@ def flash_attn_tree_with_kvcache(q, k_cache, v_cache, k, v, tree_parents,
     Position of a token: cache_seqlens + its depth.  window_size = (left, -1) keeps keys at most `left` positions back.
     rotary_cos / rotary_sin (seqlen_ro, rotary_dim / 2), both fp32 or else taken in q's dtype, turn q and k by the row of that
     position, or by rotary_positions (axes, batch, tokens) int32 with rotary_sections = pairs of each axis (see
-    rotary_axes_func, which gives the same bits).  A position outside the tables takes the nearest row.  Rows past the cache's capacity, or on a page that is not in the cache, are
-    neither written nor seen.  num_splits: 0 splits the keys so that the GPU is filled, n > 0 into at most about n parts a
-    sequence; the result depends on it by rounding alone.  Returns out (batch, tokens, nheads, headdim), or (out, softmax_lse (batch, nheads, tokens))."""
+    rotary_axes_func, which gives the same bits).  A position outside the tables takes the nearest row.  Rows past the cache's
+    capacity (at most 2^31 - 1024 rows a sequence), or on a page that is not in the cache, are neither written nor seen.
+    num_splits: 0 splits the keys so that the GPU is filled, n > 0 into at most about n parts a sequence; the result depends on
+    it by rounding alone.  Returns out (batch, tokens, nheads, headdim), or (out, softmax_lse (batch, nheads, tokens))."""
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** (-0.5)
     if isinstance(cache_seqlens, int):
