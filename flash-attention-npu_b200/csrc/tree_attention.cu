@@ -36,7 +36,6 @@ struct TreePrepArgs {
 // rotated and stacked.  Every CTA works out the tree of its sequence itself, a thread a token, by doubling: after round k a
 // token knows its 2^k nearest ancestors, so eight rounds do for any tree of 256 tokens.  (Climbing one parent a step took 18 us
 // for a chain of 64 tokens.)
-constexpr int kPrepItems = 1;
 // TT: the tables' type, T or float
 template <typename T, typename TT, bool VEC>
 __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_constant__ TreePrepArgs a) {
@@ -104,9 +103,7 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
         }
         if ((tid & 31) == 0 && (tid >> 5) < a.words) a.keys[b * a.words + (tid >> 5)] = vote;
     }
-#pragma unroll 2
-    for (int k = 0; k < kPrepItems; ++k) {
-    const int item = (blockIdx.x * kPrepItems + k) * kTreeMaxTokens + tid;
+    const int item = blockIdx.x * kTreeMaxTokens + tid;
     if (item >= a.items) return;
     const bool is_q = item >= a.items_kv, is_v = !is_q && item >= a.items_k;
     const int at = is_q ? item - a.items_kv : is_v ? item - a.items_k : item;
@@ -119,7 +116,7 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
         src = reinterpret_cast<const T*>(p.q.ptr) + (int64_t)b * p.q.stride_b + (int64_t)t * p.q.stride_s + (int64_t)h * p.q.stride_h;
         dst = reinterpret_cast<T*>(a.q_stack) + (((int64_t)b * p.hkv + hk) * nt * a.g + (int64_t)t * a.g + h % a.g) * p.d;
     } else {
-        if (!(s_stored[t >> 5] >> (t & 31) & 1)) continue;
+        if (!(s_stored[t >> 5] >> (t & 31) & 1)) return;
         const int pos = L + t;
         int64_t outer, rin;
         if (btab) {
@@ -156,7 +153,6 @@ __global__ void __launch_bounds__(kTreeMaxTokens) tree_prep_kernel(const __grid_
         }
     } else {
         for (int e = u * 16; e < min(n, u * 16 + 16); ++e) dst[e] = rd ? turn_elem<T, TT>(src, e, a.ro, rows, 1.f) : src[e];
-    }
     }
 }
 
@@ -325,7 +321,7 @@ int run_tree(const fa_tree_params& t) {
     a.items_k = p.k_new.ptr ? p.sq * p.hkv * a.uk : 0;
     a.items_kv = a.items_k + (p.k_new.ptr ? p.sq * p.hkv * a.uv : 0);
     a.items = a.items_kv + p.sq * p.hq * a.uk;
-    const dim3 grid((a.items + kPrepItems * kTreeMaxTokens - 1) / (kPrepItems * kTreeMaxTokens), p.b);
+    const dim3 grid((a.items + kTreeMaxTokens - 1) / kTreeMaxTokens, p.b);
     const bool fp32 = p.rotary_cos && t.tables_fp32;
     if (p.dtype == FA_F16) fp32 ? launch_prep<__half, float>(a, grid, st) : launch_prep<__half, __half>(a, grid, st);
     else fp32 ? launch_prep<__nv_bfloat16, float>(a, grid, st) : launch_prep<__nv_bfloat16, __nv_bfloat16>(a, grid, st);
