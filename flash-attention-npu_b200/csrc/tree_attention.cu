@@ -249,7 +249,7 @@ int check_tree(const fa_tree_params& t) {
     if (p.hq % p.hkv) return fail(FA_ERR_BAD_SHAPE, "number of heads in q must be divisible by the number of heads in k/v");
     if (p.sk > kTreeMaxRows) return fail(FA_ERR_BAD_SHAPE, "a sequence of the cache has at most 2^31 - 1024 rows");
     if (p.hkv > 65535 || p.b > 65535) return fail(FA_ERR_BAD_SHAPE, "at most 65535 sequences and KV heads");
-    if ((int64_t)p.sq * (p.hq / p.hkv) > kMaxGridY * 128 || (int64_t)p.sq * (p.hq + 2ll * p.hkv) * 16 >= (1ll << 31))
+    if ((int64_t)p.sq * (p.hq / p.hkv) > kMaxGridY * 128 || (int64_t)p.sq * (p.hq + 2ll * p.hkv) * 16 > (1ll << 31) - 512)
         return fail(FA_ERR_BAD_SHAPE, "at most 2^27 heads of tokens a sequence, 8388480 of them a KV head");
     if (p.d <= 0 || p.d > 256 || p.d != p.dv || p.d % 8) return fail(FA_ERR_BAD_SHAPE, "head dimension must be a multiple of 8 in [8, 256], the same for q, k and v");
     if (p.sq > kTreeMaxTokens) return fail(FA_ERR_UNSUPPORTED, "at most %d drafted tokens a sequence", kTreeMaxTokens);

@@ -30,7 +30,8 @@ def test_256_row_blocks_in_256_splits(d, softcap, name):
     assert ((lse[0].double() - ref).abs() <= 4e-5 * ref.abs().clamp_min(1)).all()
 
 
-@pytest.mark.parametrize("sq,hq,hkv,ok", [(256, 32767, 1, True), (256, 32768, 1, False), (256, 1 << 19, 1 << 13, False), (1, 65535 * 128, 1, True), (1, 65535 * 128 + 1, 1, False)])
+@pytest.mark.parametrize("sq,hq,hkv,ok", [(256, 32767, 1, True), (256, 32768, 1, False), (256, 1 << 19, 1 << 13, False), (1, 65535 * 128, 1, True), (1, 65535 * 128 + 1, 1, False),
+                                            (1, 65530, 32765, True), (16, 1 << 22, 1 << 21, False), (128, 65535 * 15, 65535, False), (128, 65535 * 14, 65535, True)])
 def test_more_heads_than_a_grid_holds(sq, hq, hkv, ok):
     t = params()
     t.fwd.sq, t.fwd.hq, t.fwd.hkv = sq, hq, hkv
