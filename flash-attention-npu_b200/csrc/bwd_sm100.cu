@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(608, 1) bwd_dkdv_sm100_kernel(const __grid_con
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) { tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
+    if (warp == 16) { settle_after_abort(abort_flag); tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(608, 1) bwd_dq_sm100_kernel(const __grid_const
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) { tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
+    if (warp == 16) { settle_after_abort(abort_flag); tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(64 + 128 * NB, 1) bwd_dq_from_ds_sm100_kernel(
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
+    if (warp == 1) { settle_after_abort(abort_flag); tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
 }
 
 // ------------------------------------------------------------------------------------------------------

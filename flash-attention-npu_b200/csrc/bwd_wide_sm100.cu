@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(608, 1) bwd_wide_scores_kernel(const __grid_co
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) { tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
+    if (warp == 16) { settle_after_abort(abort_flag); tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(192, 1) bwd_wide_grads_kernel(const __grid_con
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
+    if (warp == 1) { settle_after_abort(abort_flag); tc_fence_after(); tmem_dealloc(tmem, TMEM_COLS); }
 }
 
 // ------------------------------------------------------------------------------------------------------

@@ -525,6 +525,7 @@ __global__ void __launch_bounds__(320, 2) fwd_single_sm100_kernel(const __grid_c
     tc_fence_before();
     __syncthreads();
     if (warp == 8) {
+        settle_after_abort(abort_flag);
         tc_fence_after();
         tmem_dealloc(tmem, TMEM_COLS);
     }

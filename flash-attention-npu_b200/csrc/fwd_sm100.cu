@@ -570,6 +570,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel2(const __grid_constan
     tc_fence_before();
     __syncthreads();
     if (warp == 8) {
+        settle_after_abort(abort_flag);
         tc_fence_after();
         tmem_dealloc(tmem, TMEM_COLS);
     }
@@ -995,6 +996,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
     tc_fence_before();
     __syncthreads();
     if (warp == 8) {
+        settle_after_abort(abort_flag);
         tc_fence_after();
         tmem_dealloc(tmem, TMEM_COLS);
     }

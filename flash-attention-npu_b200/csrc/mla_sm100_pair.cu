@@ -456,6 +456,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mla_pai
     tc_fence_before();
     __syncthreads();
     if (warp == 12) {
+        settle_after_abort(abort_flag);
         tc_fence_after();
         tmem_dealloc(tmem, TMEM_COLS);
     }

@@ -65,6 +65,15 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     return true;
 }
 
+// Before a CTA gives its memory back: where a wait has run out, copies and matrix products that were asked for just before may
+// still be on their way into its shared and tensor memory.  They take microseconds; this waits about two milliseconds.
+constexpr long long kSettleCycles = 4000000LL;
+__device__ __forceinline__ void settle_after_abort(const volatile int* abort_flag) {
+    if (*abort_flag == 0) return;
+    const long long t0 = clock64();
+    while (clock64() - t0 < kSettleCycles) __nanosleep(1000);
+}
+
 // The same for waits that are long and not latency-critical (a producer waiting for its buffer): the warp sleeps
 // between polls so that it does not take issue slots from the warps doing arithmetic on the same scheduler.
 __device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {

@@ -581,6 +581,7 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
     tc_fence_before();
     __syncthreads();
     if (warp == 9) {
+        settle_after_abort(abort_flag);
         tc_fence_after();
         tmem_dealloc(tmem, TMEM_COLS);
     }
