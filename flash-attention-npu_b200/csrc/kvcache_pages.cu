@@ -8,6 +8,9 @@
 // The tables and counts are small (a 512 x 2048 table is 4 MB): those kernels are bound by launches and latency, and are laid
 // out to need few of both.  Copying rows is bound by HBM: 2 bytes moved a byte copied, 16-byte accesses with eight in flight a
 // thread.
+#include <algorithm>
+#include <memory>
+#include <new>
 #include "fa_utils.cuh"
 #include "fa_internal.h"
 
@@ -487,6 +490,24 @@ int check_views(const fa_pages_params& p) {
     return FA_OK;
 }
 
+// Rows that move in place may not be moved twice: no cache may begin where another does.
+int check_apart(const fa_pages_params& p) {
+    int64_t n = 0;
+    for (int i = 0; i < p.num_caches; ++i) n += p.caches[i].caches;
+    if (n < 2 || (p.num_caches == 1 && p.caches[0].stride_cache != 0)) return FA_OK;
+    constexpr int kFew = 256;
+    uint64_t few[kFew];
+    std::unique_ptr<uint64_t[]> many(n > kFew ? new (std::nothrow) uint64_t[n] : nullptr);
+    uint64_t* at = n > kFew ? many.get() : few;
+    if (!at) return fail(FA_ERR_UNSUPPORTED, "no host memory for %lld caches", (long long)n);
+    int64_t k = 0;
+    for (int i = 0; i < p.num_caches; ++i)
+        for (int c = 0; c < p.caches[i].caches; ++c) at[k++] = (uint64_t)(uintptr_t)p.caches[i].ptr + (uint64_t)c * (uint64_t)p.caches[i].stride_cache;
+    std::sort(at, at + n);
+    if (std::adjacent_find(at, at + n) != at + n) return fail(FA_ERR_UNSUPPORTED, "a cache may be given once only");
+    return FA_OK;
+}
+
 View view_of(const fa_cache_view& c) {
     View v = {reinterpret_cast<char*>(c.ptr), c.stride_cache, c.stride_page, c.stride_row, c.stride_head, c.caches, c.heads, c.segment_bytes, 1};
     if (v.heads == 1) v.head = v.seg;
@@ -608,6 +629,7 @@ int run_compact(const fa_pages_params& p) {
     if (int e = check_views(q)) return e;
     if (q.num_caches == 0) return fail(FA_ERR_BAD_SHAPE, "no caches");
     if (q.b == 0) return FA_OK;
+    if (int e = check_apart(q)) return e;
     if (!q.seqlens || !q.new_seqlens || (q.n > 0 && !q.rows)) return fail(FA_ERR_NULL, "cache_seqlens, kept or the output is null");
     if (q.new_seqlens == q.seqlens) return fail(FA_ERR_UNSUPPORTED, "the new lengths must be another tensor than the old ones");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(q.stream);

@@ -108,13 +108,6 @@ def _views(caches):
     return buf, len(caches), entries, rows, index
 
 
-def _apart(caches):
-    """Refuses a list in which one cache begins where another does: its rows would move twice."""
-    starts = [c.data_ptr() + i * c.stride(0) * c.element_size() for c in caches for i in range(c.shape[0] if c.dim() == 5 else 1)]
-    if len(set(starts)) != len(starts):
-        raise RuntimeError("a cache may be given once only")
-
-
 def _sizes(extra, page_size):
     if type(extra) is not int or not 0 <= extra < 2 ** 31:
         raise RuntimeError("extra must be a non-negative integer")
@@ -219,10 +212,7 @@ def kvcache_compact(caches, cache_seqlens, kept, counts: Optional[torch.Tensor] 
     sequence's list ends at the first entry that is not larger than the one before, or negative, or past the capacity.  The
     rows that move must lie on pages (or in cache entries) that no other sequence holds, and the caches may share no memory; a
     row on a page that is not in the cache is left out of the move.  cache_seqlens of zeros prunes whole sequences.  Returns the new lengths, int32 (batch,)."""
-    caches = (caches,) if isinstance(caches, torch.Tensor) else tuple(caches)
     views, num, entries, rows, index = _views(caches)
-    if num > 1:
-        _apart(caches)
     b = _int32("cache_seqlens", cache_seqlens, 1, index)[0]
     lens = cache_seqlens if cache_seqlens.is_contiguous() else cache_seqlens.contiguous()
     kept, (_, n), kept_stride = _read_table("kept", kept, b, index)

@@ -381,6 +381,7 @@ size_t fa_scheduler_metadata_ints(int32_t b);
  *                     increasing, counts = rows2 (null: n); ends at the first entry
  *                     out of order or past the capacity; new_seqlens = seqlens + moved.
  *                     table null: dense caches, num_pages entries of page_size rows.
+ *                     The rows move in place: a cache that is given twice is refused
  * ---------------------------------------------------------------------- */
 typedef struct {                     /* one cache, or `caches` of them stride_cache apart; strides in BYTES */
     void*   ptr;
