@@ -367,9 +367,8 @@ transforming = _transform_state()
 
 
 def has_tangent(t):
-    """True for a dual tensor, or one that a functorch transform follows: what is written into its memory reaches neither."""
-    if not transforming():
-        return False
+    """While transforming(): True for a dual tensor, or one that a functorch transform follows; what is written into its memory
+    reaches neither."""
     wrapped = getattr(getattr(torch._C, "_functorch", None), "is_functorch_wrapped_tensor", None)
     return wrapped is None or wrapped(t) or torch.autograd.forward_ad.unpack_dual(t).tangent is not None
 

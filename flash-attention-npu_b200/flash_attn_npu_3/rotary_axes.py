@@ -236,12 +236,13 @@ def rotary_axes_func(q, k, cos, sin, positions, sections=None, sections_cyclic=F
         cos, sin = cos.contiguous(), sin.contiguous()
     args = (cos, sin, positions, sections, sections_cyclic, bool(interleaved))
     if inplace:
+        transforming = capi.transforming()
         for t in (q, k):
             if t is None:
                 continue
             if torch.is_grad_enabled() and t.requires_grad:
                 raise RuntimeError("inplace rotary embedding is not differentiable: detach q and k, or leave inplace out")
-            if capi.has_tangent(t):
+            if transforming and capi.has_tangent(t):
                 raise RuntimeError("inplace rotary embedding has no forward-mode derivatives and no function transforms: leave inplace out")
             if t.stride(-1) != 1 or any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                 raise RuntimeError("inplace rotary embedding needs a contiguous last dimension and no expanded dimensions")
