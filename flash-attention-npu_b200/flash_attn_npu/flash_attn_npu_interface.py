@@ -459,6 +459,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     of (i, i + rotary_dim/2).  cache_batch_idx selects cache rows for a dense cache.
     num_splits: 0 = choose automatically, 1 = no split of the key axis, n = n splits.
     Masking, softcap, alibi and GQA as in flash_attn_func.  cache_leftpad is not supported.
+    NaN in q or in a valid row of K is not handed on reliably: where the keys are split, such a row may come out as one that saw
+    no key (zeros, softmax_lse +inf), or without the part that holds the NaN.
     Returns out, or (out, softmax_lse (batch, nheads, seqlen_q)) with return_softmax_lse.
     """
     assert k_cache.stride(-1) == 1, "k_cache must have contiguous last dimension"

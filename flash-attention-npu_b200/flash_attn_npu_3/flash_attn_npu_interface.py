@@ -316,7 +316,9 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, qv=None, rotary
     """Inference attention against a dense or paged KV cache, with optional in-place append of k / v and
     rotary embedding; same semantics as the v2 flash_attn_with_kvcache.  q may be packed (total_q, nheads,
     headdim) with cu_seqlens_q and max_seqlen_q.  scheduler_metadata (from get_scheduler_metadata) is
-    accepted; the call never synchronises with the host either way.  Returns out, or (out, softmax_lse, ...)."""
+    accepted; the call never synchronises with the host either way.  NaN in q or in a valid row of K is not handed on reliably:
+    where the keys are split, such a row may come out as one that saw no key (zeros, softmax_lse +inf), or without the part that
+    holds the NaN.  Returns out, or (out, softmax_lse, ...)."""
     assert k_cache.stride(-1) == 1, "k_cache must have contiguous last dimension"
     assert v_cache.stride(-1) == 1, "v_cache must have contiguous last dimension"
     if softmax_scale is None:

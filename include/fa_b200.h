@@ -144,11 +144,14 @@ int    fa_fwd_num_splits(const fa_fwd_params* p);
  * in front of t, or -1 for a child of the last cached row; any other value (and
  * a child of such a token) is no token: nothing is written for it, nobody sees
  * it, its output is 0 and its LSE +inf.  A window of window_left counts positions
- * L + depth.  Rows of the draft that lie past the capacity, or on a page that is
- * not in the cache, are neither written nor seen; a cached row on such a page
- * reads as zeros.
+ * L + depth.  Rows of the draft that lie past the capacity (sk, at most
+ * 2^31 - 1024), or on a page that is not in the cache, are neither written nor
+ * seen; a cached row on such a page reads as zeros.  Rows that no token sees may
+ * hold anything; V of the others must be finite.  NaN in a query, or in a row of K
+ * that it sees, makes its output and its LSE NaN.
  * Rotary turns pair i of q and k_new by table row positions[axis_of_pair[i]][b][t],
- * or by row L + depth(t) where positions is null.
+ * or by row L + depth(t) where positions is null; the tables are of q's dtype, or
+ * with tables_fp32 fp32.
  * ---------------------------------------------------------------------- */
 typedef struct {
     fa_fwd_params  fwd;
