@@ -838,7 +838,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
         const float cap_out = a.softcap * kLog2e;
         const float slope = (BIAS && a.alibi) ? a.alibi[(int64_t)b * a.alibi_sb + h] * kLog2e : 0.f;
         const float rel = (float)(qi + sk - sq);
-        // TREE: NaN when a score is, which the polynomial exponential loses
+        // TREE: NaN when a score is, which the polynomial exponential loses, as it does the inf - inf of an infinite score
         auto max3 = [](float x, float y, float z) { return TREE ? max3_nan(x, y, z) : fmaxf(fmaxf(x, y), z); };
         bool ok = true;
         for (int j = 0; j < ntiles && ok; ++j) {
@@ -949,7 +949,7 @@ __global__ void __launch_bounds__(384, 1) fwd_sm100_kernel_wide(const __grid_con
             if (full) exp_phase(std::integral_constant<int, kFwdPoly<D>>{});
             else exp_phase(std::integral_constant<int, 0>{});
             l_run += (sum_a.x + sum_b.x) + (sum_a.y + sum_b.y);
-            if (TREE && m_new != m_new) l_run = m_new;
+            if (TREE && !(m_new < INFINITY)) l_run = m_new - m_new;
         }
         if (ok) ok = mbar_wait(bar(W_O), 0, abort_flag, err, 10);
         if (TREE && !there) l_run = 0.f;

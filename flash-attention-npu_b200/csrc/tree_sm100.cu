@@ -437,7 +437,8 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
                             if (!(vis >> i & 1)) sreg[c][i] = 0xff800000u;     // -inf
                     }
                 }
-                // four independent chains of three-input maxima, NaN when a visible score is: the polynomial exponential loses it
+                // four independent chains of three-input maxima, NaN when a visible score is: the polynomial exponential loses it, and
+                // the inf - inf of an infinite score
 #pragma unroll
                 for (int c = 2 * hh; c < 2 * hh + 2; ++c) {
 #pragma unroll
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(384, 1) tree_sm100_kernel(const __grid_constan
             };
             if (full) exp_phase(std::integral_constant<int, D == 128 ? 1 : 2>{});
             else exp_phase(std::integral_constant<int, 0>{});
-            l_run = m_new != m_new ? m_new : l_run + ((sum_a.x + sum_b.x) + (sum_a.y + sum_b.y));
+            l_run = m_new < INFINITY ? l_run + ((sum_a.x + sum_b.x) + (sum_a.y + sum_b.y)) : m_new - m_new;
         }
         // ---- end of the piece ----
         float f_a = 1.f, f_b = 0.f;                          // DUAL: weights of the two groups' results

@@ -79,3 +79,25 @@ def test_a_draft_token_whose_key_is_nan(num_splits):
     c["parents"] = torch.tensor([[-1, 0, 0, 1, 2, 3, 4, -1, 7, 8]] * 2, dtype=torch.int32)
     c["k"][:, 1] = math.nan
     check(c, num_splits=num_splits)
+
+
+@pytest.mark.parametrize("kernel", KERNELS, ids=IDS)
+@pytest.mark.parametrize("num_splits", [0, 1, 4])
+@pytest.mark.parametrize("j", [0, 1, 5, 64, 127])
+def test_infinite_scores(kernel, num_splits, j):
+    """A score of +inf makes inf - inf = NaN of its row's softmax, one of -inf has no weight, and the cap makes +-cap of both."""
+    d, cap, page, pol, name = kernel
+    c = make(torch.bfloat16, d, 6, 2, [1500, 900], 9, page, seed=d + page + 4)
+    for b, tile in enumerate((5, 3)):
+        row = torch.zeros(2, d)
+        row[:, 2] = math.inf
+        c["kc"][place(c, b, tile * 128 + j)] = row.bfloat16()
+    with policy(pol):
+        out, lse, _, _ = call(c, -1, cap, num_splits)
+        assert capi.last_kernel() == name
+    ro, rl, mag = tree_attention(c["q"], c["kc"].clone(), c["vc"].clone(), c["k"], c["v"], c["parents"], c["lens"], c["table"], softcap=cap)
+    bad = (c["q"][..., 2:3] > 0).expand_as(out) & (cap == 0)
+    assert torch.equal(ro.isnan(), bad) and torch.equal(out.isnan(), bad)
+    assert ((out.double() - ro).abs()[~bad] <= out_bound(ro, mag, out.dtype)[~bad]).all()
+    fin = torch.isfinite(rl)
+    assert torch.equal(fin, torch.isfinite(lse)) and ((lse.double() - rl)[fin].abs() <= 4e-5 * rl[fin].abs().clamp_min(1)).all()
