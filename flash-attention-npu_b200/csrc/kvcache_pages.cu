@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kChunk = 4096;                 // pages whose free ones are listed together
 constexpr int kMaxPages = 1 << 24;
+constexpr int kMaxForks = 1 << 20;           // every row looks at all rows in front of it: 4096 rows 69 us, 65536 rows 1.2 ms, 2^24 a minute
 constexpr int kMaxViews = 56;                // caches (or stacks of them) of one launch: they travel as kernel parameters
 constexpr int kSmallThreads = 1024;         // of the one block that does a small call
 constexpr int kPiece = 32768;                // bytes of a page that a CTA copies at a time
@@ -584,6 +585,7 @@ int run_fork(const fa_pages_params& p) {
     if (int e = check_views(p)) return e;
     if (p.b > 0 && !p.seqlens) return fail(FA_ERR_NULL, "cache_seqlens is null");
     if (!p.missing) return fail(FA_ERR_NULL, "missing is null");
+    if (p.n > kMaxForks) return fail(FA_ERR_BAD_SHAPE, "at most 2^20 rows continue in one call");
     if (p.n > 0 && (!p.rows || !p.new_seqlens || (p.width > 0 && !p.new_table))) return fail(FA_ERR_NULL, "parents or an output is null");
     if (p.width > 0 && p.new_table == p.table && p.table) return fail(FA_ERR_UNSUPPORTED, "the new page table must be another tensor than the old one");
     if (int e = check_workspace(p, p.n)) return e;

@@ -167,7 +167,7 @@ def kvcache_free(page_refs, page_table, cache_seqlens: Optional[torch.Tensor] = 
 def kvcache_fork(caches, page_refs, page_table, cache_seqlens, parents, keep_parents=False):
     """Continue sequences several times: beam search, parallel samples.
 
-    Row i of the new table continues row parents[i] (int32 (n,)) of page_table; a number outside it makes an empty row.  Full
+    Row i of the new table continues row parents[i] (int32 (n,), n at most 2^20) of page_table; a number outside it makes an empty row.  Full
     pages are shared, their counts grow.  Of the rows that hold the same partly filled last page, the last keeps it, and the
     others get a copy of its rows in the lowest free pages, in all caches; all of them do when somebody else holds it too.
     With keep_parents the old rows stay valid (and hold their pages); without, they let go of theirs, as when beams are

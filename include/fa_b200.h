@@ -376,7 +376,8 @@ size_t fa_scheduler_metadata_ints(int32_t b);
  *                     behind the length are -1.  keep_parents = 0: the old rows let
  *                     go of all their pages.  A row number outside the old table
  *                     makes an empty row; without a free page the row ends with its
- *                     last full page and *missing counts it.
+ *                     last full page and *missing counts it.  n is at most 2^20
+ *                     (every row is compared with all in front of it).
  *   fa_pages_copy     page rows[i] -> page rows2[i] in every cache (pairs outside the
  *                     pool are skipped; a page that is written may not be named twice)
  *   fa_cache_compact  row seqlens[r] + kept[r][i] of the sequence becomes row
