@@ -389,7 +389,8 @@ def flash_attn_tree_with_kvcache(q, k_cache, v_cache, k, v, tree_parents,
     such as the -2 of a padded draft, says that there is no token: nothing is written, nobody sees it, its output is zero and
     its softmax_lse +inf; a child of such a token is none either.  Rows of V that any token sees must be finite: a tile's masked
     probabilities are exact zeros, and 0 x NaN is NaN.  Rows that no token sees may hold anything.  NaN in a query, or in a row of
-    K that it sees, makes its output and its softmax_lse NaN.
+    K that it sees, makes its output and its softmax_lse NaN; a token that sees no key (its own row has no place, nothing is
+    cached), or only scores of -inf, is answered as one that is not there.
 
     Position of a token: cache_seqlens + its depth.  window_size = (left, -1) keeps keys at most `left` positions back.
     rotary_cos / rotary_sin (seqlen_ro, rotary_dim / 2), both fp32 or else taken in q's dtype, turn q and k by the row of that

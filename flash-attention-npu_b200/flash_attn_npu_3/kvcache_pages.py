@@ -151,8 +151,7 @@ def kvcache_reserve(page_refs, page_table, cache_seqlens, page_size, extra=0):
 
 def kvcache_free(page_refs, page_table, cache_seqlens: Optional[torch.Tensor] = None, page_size=None, extra=0):
     """Let go of the pages behind cache_seqlens + extra rows (of all pages when cache_seqlens is None; page_size is only needed
-    with it), in place: their counts
-    drop by one and their entries of page_table become -1.  A page whose count is 0 stays at 0."""
+    with it), in place: their counts drop by one and their entries of page_table become -1.  A page whose count is 0 stays at 0."""
     index, pages = _pool(page_refs)
     b, width, stride = _written_table("page_table", page_table, index)
     if cache_seqlens is None:

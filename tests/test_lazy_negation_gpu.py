@@ -42,3 +42,12 @@ def test_a_negated_cache_is_refused(name):
     dev[name] = torch._neg_view(dev[name])
     with pytest.raises(RuntimeError, match="negated"):
         fa.flash_attn_tree_with_kvcache(dev["q"], dev["kc"], dev["vc"], dev["k"], dev["v"], dev["parents"], cache_seqlens=dev["lens"], page_table=dev["table"])
+
+
+def test_rotary_in_place_on_negated_q_and_k():
+    """The memory is turned: the negative of the turned is the turned negative, bit for bit."""
+    q, k, cos, sin, pos = inputs(torch.bfloat16, (2, 4), 4, 2, 64, 48, 1, torch.float32)
+    want = fa.rotary_axes_func(-q, -k, cos, sin, pos)
+    a, b = q.clone(), k.clone()
+    here = fa.rotary_axes_func(torch._neg_view(a), torch._neg_view(b), cos, sin, pos, inplace=True)
+    assert all(torch.equal(x, y) for x, y in zip(want, here)) and torch.equal(-a, want[0]) and torch.equal(-b, want[1])
